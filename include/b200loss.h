@@ -413,6 +413,78 @@ int b200_pc_softmax_ce_scaled(const void *logits, const int64_t *labels, const f
                               void *losses, void *grad_logits, const void *denom, int64_t N,
                               int64_t C, int64_t M, int dtype, int64_t ignore_index, void *stream);
 
+/* ------------------------------------------- log probabilities of given tokens ---
+ * No counterpart in the reference.  Rows of a language model's logits: row r starts at element
+ * r * stride of `logits` (stride >= V for a padded vocabulary, any alignment), at most 2^28 - 1 rows
+ * of at most 2^30 logits; temperature T in [1e-4, 1e4].  With z = x / T and p = softmax(z):
+ *   logprobs[r] = log p[tokens[r]]        entropy[r] = -sum_j p_j log p_j            (floats)
+ *   top_logprobs / top_tokens [rows, top_k]: the top_k (<= 128, <= V) largest, in order; equal logits
+ *       by index, NaN in front (top_k == 0: pass null)
+ *   stats: float[rows][4], 16-byte aligned, what the backward call needs (null: none wanted)
+ * A row whose token is ignore_index is not read: 0, 0, 0 and -1, and a zero gradient.  A token outside
+ * [0, V) gives NaN (also in the gradient); a row of -inf alone -inf, entropy 0 and a zero gradient.
+ * backward: grad_logits [rows, V] contiguous =
+ *   (d_logprobs[r] (1[j = token] - p_j) - d_entropy[r] p_j (log p_j + entropy[r])) / T; either upstream
+ *   gradient may be null. */
+int b200_token_logprobs(const void *logits, const int64_t *tokens, float *logprobs, float *entropy,
+                        void *stats, float *top_logprobs, int64_t *top_tokens, int64_t rows, int64_t V,
+                        int64_t stride, int dtype, int top_k, float temperature, int64_t ignore_index,
+                        void *stream);
+int b200_token_logprobs_backward(const void *logits, const int64_t *tokens, const void *stats,
+                                 const float *d_logprobs, const float *d_entropy, void *grad_logits,
+                                 int64_t rows, int64_t V, int64_t stride, int dtype, float temperature,
+                                 int64_t ignore_index, void *stream);
+
+/* ------------------------------------- distillation from a teacher's alternatives ---
+ * No counterpart in the reference.  Logits as above against lists of K <= 128 tokens with log
+ * probabilities (top_tokens, top_logprobs [rows, K], as b200_token_logprobs writes them):
+ *   w = softmax(top_logprobs[r, :])     loss[r] = sum_k w_k (log w_k - log p[top_tokens[r, k]])
+ * Entries with a negative token do not exist, the same token twice adds up.  A row without an entry of
+ * finite log probability is not read: loss 0, gradient 0, not counted.  A token >= V gives NaN.
+ *   forward : losses float[rows] and / or out (reduction record: sum, count, mean over the counted rows)
+ *   backward: grad_logits [rows, V] contiguous = d_loss (p_j - w_j) / T, d_loss one float per row
+ *       (per_row) or one for all, divided by *count (device double, e.g. the record's; may be null);
+ *       scratch: what the forward call of the same inputs left
+ *   step    : out and the final gradient (mean: divided by the number of counted rows) from ONE read of
+ *       the logits; b200_top_distill_step_path: 1 when the layout has it (float32 / bfloat16, gradient
+ *       rows at the logits' place within 16 bytes, rows of up to 1.6 MB).  float16 has none: there the
+ *       upstream gradient (loss scaling) has to come in before the one rounding.  Backward of the step is
+ *       b200_rescale_gradient.
+ * scratch: b200_top_distill_scratch_bytes(rows, K) bytes, 16-byte aligned, contents irrelevant. */
+size_t b200_top_distill_scratch_bytes(int64_t rows, int K);
+int b200_top_distill_forward(const void *logits, const int64_t *top_tokens, const float *top_logprobs,
+                             float *losses, void *out, void *scratch, size_t scratch_bytes,
+                             int64_t rows, int64_t V, int64_t stride, int dtype, int K,
+                             float temperature, void *stream);
+int b200_top_distill_backward(const void *logits, const int64_t *top_tokens, const void *scratch,
+                              size_t scratch_bytes, const float *d_loss, int per_row, const void *count,
+                              void *grad_logits, int64_t rows, int64_t V, int64_t stride, int dtype,
+                              int K, float temperature, void *stream);
+int b200_top_distill_step_path(const void *logits, const void *grad_logits, int64_t rows, int64_t V,
+                               int64_t stride, int dtype);
+int b200_top_distill_step(const void *logits, const int64_t *top_tokens, const float *top_logprobs,
+                          void *grad_logits, void *out, void *scratch, size_t scratch_bytes,
+                          int64_t rows, int64_t V, int64_t stride, int dtype, int K, float temperature,
+                          int mean, void *stream);
+
+/* ------------------------------------------------------------------ layer norm ---
+ * Rows of D contiguous elements (row r at element r * stride of x, any alignment), at most 2^31 - 1 rows
+ * of 2^30 elements; weight and bias (either may be null: 1 and 0) have the rows' type or float32
+ * (param_dtype).
+ *   y [rows, D] contiguous = (x - mean) / sqrt(var + eps) * weight + bias
+ *   stats: float[rows][2] = {mean, 1 / sqrt(var + eps)}, what the backward call needs (null: none wanted)
+ * backward: dx [rows, D] contiguous; dweight, dbias [D] in the parameters' type, the sums over all rows
+ *   in a fixed order (either may be null; scratch, b200_layer_norm_scratch_bytes(rows, D) bytes on a
+ *   16-byte address, contents irrelevant, is needed for them only). */
+int b200_layer_norm(const void *x, const void *weight, const void *bias, void *y, void *stats,
+                    int64_t rows, int64_t D, int64_t stride, int dtype, int param_dtype, float eps,
+                    void *stream);
+size_t b200_layer_norm_scratch_bytes(int64_t rows, int64_t D);
+int b200_layer_norm_backward(const void *x, const void *weight, const void *stats, const void *dy, void *dx,
+                             void *dweight, void *dbias, void *scratch, size_t scratch_bytes,
+                             int64_t rows, int64_t D, int64_t stride, int64_t dy_stride, int dtype,
+                             int param_dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

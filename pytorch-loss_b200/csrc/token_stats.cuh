@@ -1,0 +1,559 @@
+// The forward kernel of the log-probability and distillation operators (token_logprobs.cu, top_distill.cu) and the
+// kernel that writes a gradient from a row's statistics.  Formulas: token_rows.cuh.
+#pragma once
+#include "token_rows.cuh"
+
+namespace b200 {
+namespace {
+
+// kTokens: one given token per row, entropy, best alternatives.  kList: a list of tokens with weights per row.
+enum TokenMode { kTokens = 0, kList = 1 };
+
+struct TokenParams {
+    const void *x;              // logits: row r starts at element r * stride
+    int64_t stride, rows;
+    int V;
+    float c, inv_t;             // log2(e) / temperature, 1 / temperature
+    const int64_t *ids;         // kTokens: [rows]; kList: [rows, K]
+    const float *weight;        // kList: [rows, K], a row sums to 1, 0 where nothing is asked
+    const float *base;          // kList: [rows], sum of w log w; +inf: nothing is asked of the row, NaN: a bad token
+    int64_t ignore;
+    int K;                      // kTokens: alternatives; kList: length of the lists
+    float *out, *entropy;       // log probabilities and entropies, or losses
+    float4 *stats;              // {m, 1 / s, u / s, log2 s} for the gradient (may be null)
+    float *top_logprobs;
+    int64_t *top_tokens;
+    int parts;                  // blocks of a cluster that share a row
+};
+
+// ---- alternatives
+// Order: larger logits first, the lower index first among equals (-0 = +0), NaN in front of everything.  A key holds
+// that order in one unsigned number: the value's bits made monotone, above the inverted index.
+__device__ __forceinline__ unsigned value_key(float x) {
+    unsigned b = __float_as_uint(x);
+    if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+    if ((b << 1) == 0u) b = 0u;
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(unsigned k) {
+    return k == 0xffffffffu ? __uint_as_float(0x7fc00000u)
+                            : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ unsigned long long top_key(float x, int j) {
+    return (static_cast<unsigned long long>(value_key(x)) << 32) | unsigned(~j);
+}
+
+template <int G> __device__ __forceinline__ void group_sync() {
+    if (G == 32) __syncwarp();
+    else __syncthreads();
+}
+
+// Candidates that a group of G threads keeps.  32 lanes: their lists are at most 32 long (largest() below).
+template <int G> constexpr int kCandidates = G == 32 ? 256 : 1024;
+
+template <int G, bool TOP> struct TokenShared {
+    float m[G / 32], s[G / 32], u[G / 32];
+    float joined[3];                                     // this block's share of the row, for the cluster
+    float log2s, row_m;
+    int count;
+    unsigned bound;
+    unsigned short keys[TOP ? G : 1];
+    unsigned hist[TOP ? 256 : 1];
+    unsigned long long cand[TOP ? kCandidates<G> : 1];
+    unsigned long long best[TOP ? kMaxList : 1];
+};
+
+// The smallest key among the `want` largest of the part (0 if the part has no more than that): eight passes over the
+// part, one digit of the 64-bit keys each.  Only for parts whose candidates do not fit: logits that agree at
+// thousands of places, or lie so that a few threads see all the large ones.
+template <typename T, int G, bool TOP>
+__device__ __noinline__ unsigned long long exact_bound(const T *row, RowPart part, int t, int want,
+                                                       TokenShared<G, TOP> &sh) {
+    if (part.last - part.first <= want) return 0ull;
+    unsigned long long prefix = 0ull;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        for (int i = t; i < 256; i += G) sh.hist[i] = 0u;
+        group_sync<G>();
+        for (int base = part.first; base < part.last; base += G) {
+            const int j = base + t;
+            const unsigned long long key = j < part.last ? top_key(to_f32(row[j]), j) : 0ull;
+            const bool in = j < part.last && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+            const unsigned digit = unsigned(key >> shift) & 255u;
+            const unsigned live = __ballot_sync(0xffffffffu, in);
+            if (live == 0u) continue;
+            const unsigned first = __shfl_sync(0xffffffffu, digit, __ffs(live) - 1);
+            if (__all_sync(0xffffffffu, !in || digit == first)) {       // (equal logits: one addition for all lanes)
+                if ((t & 31) == 0) atomicAdd(&sh.hist[first], unsigned(__popc(live)));
+            } else if (in) {
+                atomicAdd(&sh.hist[digit], 1u);
+            }
+        }
+        group_sync<G>();
+        // from the largest digit down: the one at which `want` is reached (every warp finds the same)
+        unsigned mine = 0u;
+        const int lane = t & 31;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine += sh.hist[255 - lane * 8 - i];
+        unsigned upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned other = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += other;
+        }
+        const int owner = __ffs(__ballot_sync(0xffffffffu, upto >= unsigned(want))) - 1;
+        int digit = 0, left = 0;
+        if (lane == owner) {
+            left = want - int(upto - mine);
+            digit = 255 - lane * 8;
+            while (int(sh.hist[digit]) < left) left -= int(sh.hist[digit--]);
+        }
+        want = __shfl_sync(0xffffffffu, left, owner);
+        prefix |= static_cast<unsigned long long>(__shfl_sync(0xffffffffu, digit, owner)) << shift;
+        group_sync<G>();
+    }
+    return prefix;
+}
+
+// sh.best[0..K) = the K largest keys of the part in order, 0 behind its end.  `m`: the largest logit of each thread.
+//
+// The K-th largest of the threads' maxima is a lower bound of the K-th largest logit, so only the few threads whose
+// maximum reaches it read their logits again (from L2), and what they keep is little more than K.  The bound is taken
+// to the upper 16 bits of the keys: a warp finds it in 16 steps.  The order among the kept is a count of larger keys.
+template <typename T, int G, bool TOP, typename Load>
+__device__ __forceinline__ void largest(const T *row, const RowPart &part, int t, float m, int K,
+                                        TokenShared<G, TOP> &sh, Load load) {
+    constexpr int N = TokenVec<T>::N, PER = G / 32, CAP = kCandidates<G>;
+    const unsigned key = value_key(m) >> 16;
+    sh.keys[t] = static_cast<unsigned short>(key);
+    if (t == 0) sh.count = 0;
+    group_sync<G>();
+    if (t < 32) {
+        unsigned k[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) k[i] = sh.keys[t + 32 * i];
+        unsigned bound = 0u;
+#pragma unroll 1
+        for (int bit = 15; bit >= 0; --bit) {
+            const unsigned trial = bound | (1u << bit);
+            unsigned n = 0u;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) n += k[i] >= trial ? 1u : 0u;
+            if (__reduce_add_sync(0xffffffffu, n) >= unsigned(K)) bound = trial;
+        }
+        if (t == 0) sh.bound = bound;
+    }
+    group_sync<G>();
+    const unsigned bound = sh.bound;
+    auto keep = [&](float x, int j) {
+        const unsigned long long k = top_key(x, j);
+        if (unsigned(k >> 48) >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < CAP) sh.cand[at] = k;
+        }
+    };
+    if (key >= bound) {
+        for (int i = part.body + t * N; i < part.body_end; i += kTokenUnroll * G * N) {
+            uint4 v[kTokenUnroll];
+#pragma unroll
+            for (int k = 0; k < kTokenUnroll; ++k) {
+                const int64_t at = i + int64_t(k) * (G * N);
+                if (at < part.body_end) v[k] = load(int(at));
+            }
+#pragma unroll
+            for (int k = 0; k < kTokenUnroll; ++k) {
+                const int64_t at = i + int64_t(k) * (G * N);
+                if (at < part.body_end) {
+#pragma unroll
+                    for (int h = 0; h < N / 2; ++h) {
+                        const float2 x = TokenVec<T>::pair(v[k], h);
+                        keep(x.x, int(at) + 2 * h);
+                        keep(x.y, int(at) + 2 * h + 1);
+                    }
+                }
+            }
+        }
+        if (t < ragged_count(part)) {
+            const int j = ragged_index(part, t);
+            keep(to_f32(row[j]), j);
+        }
+    }
+    group_sync<G>();
+    int n = sh.count;
+    if (n > CAP) {
+        const unsigned long long least = exact_bound<T, G, TOP>(row, part, t, K, sh);
+        if (t == 0) sh.count = 0;
+        group_sync<G>();
+        for (int j = part.first + t; j < part.last; j += G) {
+            const unsigned long long k = top_key(to_f32(row[j]), j);
+            if (k >= least) sh.cand[atomicAdd(&sh.count, 1)] = k;       // (at most K <= kMaxList of them)
+        }
+        group_sync<G>();
+        n = sh.count;
+    }
+    for (int i = t; i < K; i += G)
+        if (i >= n) sh.best[i] = 0ull;
+    for (int i = t; i < n; i += G) {
+        const unsigned long long k = sh.cand[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += sh.cand[j] > k ? 1 : 0;
+        if (rank < K) sh.best[rank] = k;
+    }
+    group_sync<G>();
+}
+
+__device__ __forceinline__ void write_alternative(const TokenParams &p, int64_t row, int i, unsigned long long key,
+                                                  float m, float log2s, bool nothing) {
+    const float x = key_value(unsigned(key >> 32));
+    p.top_logprobs[row * p.K + i] = nothing ? -INFINITY : log_prob(x, m, p.inv_t, log2s);
+    p.top_tokens[row * p.K + i] = int64_t(~unsigned(key));
+}
+
+// G threads to a row (32: eight rows to a block), or the G threads of each of `parts` blocks.
+// Bound: HBM, the logits once; instruction issue and the 16 exponentials a clock of an SM are next (16-bit logits
+// take 11.6 of them at HBM speed).
+template <typename T, int G, int MODE, bool TOP>
+__global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const TokenParams p) {
+    constexpr bool ENTROPY = MODE == kTokens;
+    constexpr int WARPS = G / 32, GROUPS = G == 32 ? 8 : 1;
+    __shared__ TokenShared<G, TOP> shared[GROUPS];
+    const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, lane = threadIdx.x & 31;
+    TokenShared<G, TOP> &sh = shared[G == 32 ? threadIdx.x >> 5 : 0];
+    const int parts = G == 32 ? 1 : p.parts;
+    const int rank = G == 32 ? 0 : int(blockIdx.x % unsigned(parts));
+    const int64_t r = G == 32 ? int64_t(blockIdx.x) * GROUPS + (threadIdx.x >> 5) : int64_t(blockIdx.x / unsigned(parts));
+    if (r >= p.rows) return;
+    const T *row = static_cast<const T *>(p.x) + r * p.stride;
+
+    // rows that are not asked for are not read (the blocks of a cluster leave together)
+    int64_t token = 0;
+    float given = 0.f;
+    bool bad = false;
+    if (MODE == kTokens) {
+        token = p.ids[r];
+        if (token == p.ignore) {
+            if (rank == 0) {
+                if (t == 0) {
+                    p.out[r] = 0.f;
+                    p.entropy[r] = 0.f;
+                }
+                if (TOP)
+                    for (int i = t; i < p.K; i += G) {
+                        p.top_logprobs[r * p.K + i] = 0.f;
+                        p.top_tokens[r * p.K + i] = -1;
+                    }
+            }
+            return;
+        }
+        bad = token < 0 || token >= p.V;
+        if (rank == 0 && t == 0 && !bad) given = to_f32(row[token]);
+    } else {
+        given = p.base[r];
+        if (given == INFINITY) {
+            if (rank == 0 && t == 0) p.out[r] = 0.f;
+            return;
+        }
+    }
+
+    const RowPart part = row_part(row, p.V, rank, parts);
+    auto load = [row](int i) { return ld_stream16<uint4>(row + i); };
+    RowStat<ENTROPY> st;
+    st.init();
+    scan_part<T, G, ENTROPY>(row, part, t, p.c, st, load);
+    const float own_max = st.m;
+    st.join_warp(p.c);
+    if (G > 32) {
+        if (lane == 0) {
+            sh.m[t >> 5] = st.m;
+            sh.s[t >> 5] = st.s;
+            if (ENTROPY) sh.u[t >> 5] = st.u;
+        }
+        __syncthreads();
+        st.init();
+        if (lane < WARPS) {
+            st.m = sh.m[lane];
+            st.s = sh.s[lane];
+            if (ENTROPY) st.u = sh.u[lane];
+        }
+        st.join_warp(p.c);
+    }
+    if constexpr (TOP) largest<T, G, TOP>(row, part, t, own_max, p.K, sh, load);
+
+    if (G > 32 && parts > 1) {
+        namespace cg = cooperative_groups;
+        cg::cluster_group cluster = cg::this_cluster();
+        if (t == 0) {
+            sh.joined[0] = st.m;
+            sh.joined[1] = st.s;
+            sh.joined[2] = ENTROPY ? st.u : 0.f;
+        }
+        cluster.sync();
+        if (rank == 0) {
+            st.init();
+            if (lane < parts) {
+                const float *other = cluster.map_shared_rank(&sh.joined[0], lane);
+                st.m = other[0];
+                st.s = other[1];
+                if (ENTROPY) st.u = other[2];
+            }
+            st.join_warp(p.c);
+            if constexpr (TOP) {
+                for (int i = t; i < parts * p.K; i += G)
+                    sh.cand[i] = cluster.map_shared_rank(&sh.best[0], i / p.K)[i % p.K];
+                __syncthreads();
+                for (int i = t; i < parts * p.K; i += G) {
+                    const unsigned long long k = sh.cand[i];
+                    int place = 0;
+                    for (int j = 0; j < parts * p.K; ++j) place += sh.cand[j] > k ? 1 : 0;
+                    if (k != 0ull && place < p.K)
+                        write_alternative(p, r, place, k, reference_of(st.m), log2f(st.s), st.s == 0.f);
+                }
+            }
+        }
+        cluster.sync();                                     // (nobody leaves while its memory is read)
+        if (rank != 0) return;
+    } else if constexpr (TOP) {
+        for (int i = t; i < p.K; i += G)
+            write_alternative(p, r, i, sh.best[i], reference_of(st.m), log2f(st.s), st.s == 0.f);
+    }
+
+    const float m = reference_of(st.m), log2s = log2f(st.s);
+    const bool nothing = st.s == 0.f;                       // a row of -inf
+    if (MODE == kTokens) {
+        if (t == 0) {
+            const float mean = nothing ? 0.f : st.u / st.s;
+            p.out[r] = bad ? __int_as_float(0x7fc00000) : nothing ? -INFINITY
+                                                                  : log_prob(given, m, p.inv_t, log2s);
+            p.entropy[r] = nothing ? 0.f : max_nan(kTokenLn2 * (log2s - mean), 0.f);
+            if (p.stats) p.stats[r] = make_float4(m, nothing ? 0.f : 1.f / st.s, mean, log2s);
+        }
+    } else if (t < 32) {
+        // sum of w (log w - log p) over the list; `given` holds the sum of w log w
+        float part_loss = 0.f;
+        for (int i = lane; i < p.K; i += 32) {
+            const float w = p.weight[r * p.K + i];
+            if (w > 0.f) {                                  // (0 for tokens that do not exist)
+                const float x = to_f32(row[p.ids[r * p.K + i]]);
+                part_loss = fmaf(-w, nothing ? -INFINITY : log_prob(x, m, p.inv_t, log2s), part_loss);
+            }
+        }
+        part_loss = warp_sum(part_loss);
+        if (lane == 0) {
+            p.out[r] = given + part_loss;
+            if (p.stats) p.stats[r] = make_float4(m, nothing ? 0.f : 1.f / st.s, 0.f, log2s);
+        }
+    }
+}
+
+// ---- gradient from the statistics
+// kTokens: g_j = e_j (A + B z_j) + dl [j = token] / T,  A = -(dl - dh ln2 u / s) / (s T),  B = -dh ln2 / (s T)
+// kList:   g_j = scale (p_j - w_j) / T
+// where e_j = 2^z_j; elementwise: reads the logits once, writes the gradient once, no barrier before the last list
+// step.  A row of -inf alone gets zeros, one that is not asked for too (without being read).
+struct TokenGradParams {
+    const void *x;
+    void *grad;                 // [rows, V], contiguous
+    int64_t stride, rows;
+    int V;
+    float c, inv_t;
+    const int64_t *ids;
+    const float *weight, *base;
+    const float4 *stats;
+    const float *d_out;         // upstream gradient of the log probabilities or losses: [rows] or one value
+    int d_out_step;             // 1: one per row, 0: one for all
+    const float *d_entropy;     // [rows] or null
+    const double *count;        // kList: divisor (null: none)
+    int64_t ignore;
+    int K;
+    int chunks;                 // blocks per row
+};
+
+// G threads to a chunk of G * kTokenUnroll vectors.  ALIGNED: logits and gradient rows start at the same place within
+// 16 bytes, so that whole vectors of one are whole vectors of the other; else the logits are read one by one.
+template <typename T, int G, int MODE, bool ALIGNED>
+__global__ void __launch_bounds__(256) token_grad_kernel(const TokenGradParams p) {
+    constexpr int N = TokenVec<T>::N;
+    constexpr int GROUPS = 256 / G;
+    const int t = threadIdx.x % G;
+    const int64_t unit = int64_t(blockIdx.x) * GROUPS + threadIdx.x / G;
+    const int64_t r = unit / p.chunks;
+    const int chunk = int(unit % p.chunks);
+    if (r >= p.rows) return;
+    const T *x = static_cast<const T *>(p.x) + r * p.stride;
+    T *g = static_cast<T *>(p.grad) + r * int64_t(p.V);
+
+    float A = 0.f, B = 0.f, at_token = 0.f, m = 0.f;
+    int token = -1;
+    bool zero = false;
+    if (MODE == kTokens) {
+        const int64_t id = p.ids[r];
+        zero = id == p.ignore;
+        if (!zero) {
+            const float4 st = p.stats[r];
+            float dl = p.d_out ? p.d_out[r * p.d_out_step] : 0.f;
+            const float dh = p.d_entropy ? p.d_entropy[r] : 0.f;
+            const bool bad = id < 0 || id >= p.V;
+            if (bad) dl = __int_as_float(0x7fc00000);
+            m = st.x;
+            B = -dh * kTokenLn2 * st.y * p.inv_t;
+            A = -(dl - dh * kTokenLn2 * st.z) * st.y * p.inv_t;
+            token = bad ? -1 : int(id);
+            at_token = dl * p.inv_t;
+            zero = st.y == 0.f && !bad;
+        }
+    } else {
+        const float base = p.base[r];
+        zero = base == INFINITY;
+        if (!zero) {
+            const float4 st = p.stats[r];
+            float scale = p.d_out[r * p.d_out_step] * p.inv_t;
+            if (p.count) scale = float(double(scale) / *p.count);
+            if (base != base) scale = base;
+            m = st.x;
+            A = scale * st.y;
+            at_token = -scale;
+            zero = st.y == 0.f;
+        }
+    }
+
+    const RowPart part = row_part(static_cast<const T *>(g), p.V, chunk, p.chunks);
+    const pk_t negm = psplat(-m), cc = psplat(p.c), aa = psplat(A), bb = psplat(B);
+    auto one = [&](float v) {                               // without what a given token adds
+        const float z = max_nan((v - m) * p.c, kTokenFloor), e = ex2f(z);
+        return e * fmaf(B, z, A);
+    };
+    for (int i = part.body + t * N; i < part.body_end; i += kTokenUnroll * G * N) {
+        uint4 v[kTokenUnroll];
+#pragma unroll
+        for (int k = 0; k < kTokenUnroll; ++k) {
+            const int64_t at = i + int64_t(k) * (G * N);
+            v[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (!zero && at < part.body_end) {
+                if (ALIGNED) {
+                    v[k] = ld_stream16<uint4>(x + at);
+                } else {
+                    T e[N];
+#pragma unroll
+                    for (int h = 0; h < N; ++h) e[h] = x[at + h];
+                    memcpy(&v[k], e, 16);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kTokenUnroll; ++k) {
+            const int64_t at = i + int64_t(k) * (G * N);
+            if (at >= part.body_end) break;
+            if (!zero) {
+                float2 d[N / 2];
+#pragma unroll
+                for (int h = 0; h < N / 2; ++h) {
+                    float2 z = upk2(pmul(padd(pk2(TokenVec<T>::pair(v[k], h)), negm), cc));
+                    z.x = max_nan(z.x, kTokenFloor);
+                    z.y = max_nan(z.y, kTokenFloor);
+                    const pk_t zz = pk2(z);
+                    const pk_t e = pex2(zz);
+                    d[h] = upk2(MODE == kTokens ? pmul(e, pfma(bb, zz, aa)) : pmul(e, aa));
+                }
+                if (MODE == kTokens && unsigned(token - int(at)) < unsigned(N)) {
+                    const int w = token - int(at);
+#pragma unroll
+                    for (int h = 0; h < N / 2; ++h) {
+                        if (w == 2 * h) d[h].x += at_token;
+                        if (w == 2 * h + 1) d[h].y += at_token;
+                    }
+                }
+                v[k] = TokenVec<T>::pack(d);
+            }
+            st_stream16(g + at, v[k]);
+        }
+    }
+    if (t < ragged_count(part)) {
+        const int j = ragged_index(part, t);
+        const float d = zero ? 0.f : one(to_f32(x[j]));
+        g[j] = from_f32<T>(MODE == kTokens && !zero && j == token ? d + at_token : d);
+    }
+    if (MODE == kList && !zero) {
+        group_sync<G>();                                    // (what the list changes has been written)
+        for (int i = t; i < p.K; i += G) {
+            const float w = p.weight[r * p.K + i];
+            const int64_t j = p.ids[r * p.K + i];
+            if (w > 0.f && j >= part.first && j < part.last)
+                g[j] = from_f32<T>(fmaf(at_token, w, one(to_f32(x[j]))));
+        }
+    }
+}
+
+// ---- launches
+
+// How many threads share a row and over how many blocks it is split.  Rows of up to 4 KB are a warp's (no barrier;
+// lists of alternatives up to 32).  Longer rows are a block's; with few rows they are split over the blocks of a
+// cluster, as long as all of them run at once and every thread still has a vector.
+inline int row_parts(int64_t rows, int64_t V, int dtype) {
+    const int64_t vectors = row_vectors(V, dtype), room = int64_t(sm_count()) * 8;
+    int parts = 1;
+    while (parts < kMaxCluster && rows * parts * 2 <= room && vectors / (parts * 2) >= 256) parts *= 2;
+    return parts;
+}
+
+template <typename T, int MODE, bool TOP> int launch_stats(const TokenParams &prm, int dtype, cudaStream_t stream) {
+    TokenParams p = prm;
+    const char *what = "token statistics kernel launch";
+    if (p.rows == 0) return B200_OK;
+    if (p.V * int64_t(sizeof(T)) <= 4096 && !(TOP && p.K > 32)) {
+        p.parts = 1;
+        return launch_cluster(token_stats_kernel<T, 32, MODE, TOP>, (p.rows + 7) / 8, 256, 0, 1, false, stream, what, p);
+    }
+    p.parts = row_parts(p.rows, p.V, dtype);
+    return launch_cluster(token_stats_kernel<T, 256, MODE, TOP>, p.rows * p.parts, 256, 0, p.parts, false, stream, what,
+                          p);
+}
+
+template <typename T, int MODE> int launch_grad(const TokenGradParams &prm, int dtype, cudaStream_t stream) {
+    TokenGradParams p = prm;
+    const char *what = "token gradient kernel launch";
+    if (p.rows == 0) return B200_OK;
+    const int64_t vectors = row_vectors(p.V, dtype);
+    const int64_t shift = int64_t((reinterpret_cast<uintptr_t>(p.x) - reinterpret_cast<uintptr_t>(p.grad)) & 15);
+    const bool aligned = shift == 0 && (p.rows == 1 || ((p.stride - p.V) * int64_t(sizeof(T))) % 16 == 0);
+    if (vectors <= 32 * kTokenUnroll) {
+        p.chunks = 1;
+        const int64_t grid = (p.rows + 7) / 8;
+        return aligned ? launch_cluster(token_grad_kernel<T, 32, MODE, true>, grid, 256, 0, 1, false, stream, what, p)
+                       : launch_cluster(token_grad_kernel<T, 32, MODE, false>, grid, 256, 0, 1, false, stream, what, p);
+    }
+    p.chunks = int((vectors + 256 * kTokenUnroll - 1) / (256 * kTokenUnroll));
+    const int64_t grid = p.rows * p.chunks;
+    if (grid > 0x7fffffff) {
+        set_error("%s: %lld rows of %d logits are more than one launch covers", what, (long long)p.rows, p.V);
+        return B200_ERR_UNSUPPORTED;
+    }
+    return aligned ? launch_cluster(token_grad_kernel<T, 256, MODE, true>, grid, 256, 0, 1, false, stream, what, p)
+                   : launch_cluster(token_grad_kernel<T, 256, MODE, false>, grid, 256, 0, 1, false, stream, what, p);
+}
+
+// What every entry point of the family refuses.
+inline int check_rows(const char *who, const void *x, int64_t rows, int64_t V, int64_t stride, int dtype, float temperature) {
+    if (rows < 0 || V < 1 || (rows > 1 && stride < 0)) {
+        set_error("%s: need rows >= 0, V >= 1 and stride >= 0", who);
+        return B200_ERR_ARG;
+    }
+    if (rows > 0x0fffffff || V > (int64_t(1) << 30)) {
+        set_error("%s: at most 2^28 - 1 rows and 2^30 logits per row", who);
+        return B200_ERR_UNSUPPORTED;
+    }
+    if (!dtype_known(dtype)) {
+        set_error("%s: unknown dtype code %d", who, dtype);
+        return B200_ERR_ARG;
+    }
+    if (!(temperature >= 1e-4f && temperature <= 1e4f)) {
+        set_error("%s: the temperature must lie between 1e-4 and 1e4", who);
+        return B200_ERR_ARG;
+    }
+    if (rows > 0 && (!x || (reinterpret_cast<uintptr_t>(x) & (dtype_size(dtype) - 1)))) {
+        set_error("%s: the logits are null or not aligned to their type", who);
+        return B200_ERR_ARG;
+    }
+    return B200_OK;
+}
+
+}  // namespace
+}  // namespace b200

@@ -72,6 +72,16 @@ SIGNATURES = {
     "b200_pc_softmax_ce_scaled": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _i64, _vp]),
     "b200_ohem_workspace_bytes": (_sz, [_i64, _i64]),
     "b200_ohem_label": (_int, [_vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _int, _i64, _f32, _i64, _vp]),
+    "b200_token_logprobs": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _f32, _i64, _vp]),
+    "b200_token_logprobs_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _f32, _i64, _vp]),
+    "b200_layer_norm": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _f32, _vp]),
+    "b200_layer_norm_scratch_bytes": (_sz, [_i64, _i64]),
+    "b200_layer_norm_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _i64, _int, _int, _vp]),
+    "b200_top_distill_scratch_bytes": (_sz, [_i64, _int]),
+    "b200_top_distill_forward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _int, _int, _f32, _vp]),
+    "b200_top_distill_backward": (_int, [_vp, _vp, _vp, _sz, _vp, _int, _vp, _vp, _i64, _i64, _i64, _int, _int, _f32, _vp]),
+    "b200_top_distill_step_path": (_int, [_vp, _vp, _i64, _i64, _i64, _int]),
+    "b200_top_distill_step": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _int, _int, _f32, _int, _vp]),
 }
 
 _lib = None
@@ -228,6 +238,23 @@ def split_shape(logits, labels=None):
         if labels.dtype != torch.int64:
             raise RuntimeError("labels must be int64, got %s" % labels.dtype)
     return n, c, m
+
+
+def as_rows(t):
+    """(tensor whose memory the kernels read, rows, n, elements from row to row) of a tensor [..., n].  Rows may lie
+    apart (a slice of a padded storage, a permuted view) as long as one stride describes them; anything else is copied."""
+    if t.dim() < 1 or t.shape[-1] == 0:
+        raise RuntimeError("need a tensor [..., n] with n > 0, got shape %s" % (tuple(t.shape),))
+    n = t.shape[-1]
+    if n > 1 and t.stride(-1) != 1:
+        t = t.contiguous()
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    elif t.dim() > 2:
+        t = t.flatten(0, -2)
+        if n > 1 and t.stride(-1) != 1:
+            t = t.contiguous()
+    return t, t.shape[0], n, t.stride(0)
 
 
 def scalar_gradient(grad_output):

@@ -1,0 +1,110 @@
+"""Layer norm over the last dimension on the B200 CUDA library: forward in one read of the rows, backward in one read
+of rows and upstream gradient that also leaves the sums for weight and bias.
+"""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _cabi
+
+
+def _check(x, weight, bias, eps):
+    dev = _cabi.require_cuda(x, weight, bias)
+    dt = _cabi.dtype_code(x)
+    par = None
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if x.dim() < 1 or t.dim() != 1 or t.shape[0] != x.shape[-1]:
+            raise RuntimeError("%s of shape %s does not match rows of %s" % (name, tuple(t.shape), tuple(x.shape)))
+        if t.dtype not in (x.dtype, torch.float32) or (par is not None and t.dtype != par):
+            raise RuntimeError("weight and bias must both be float32 or both %s, got %s" % (x.dtype, t.dtype))
+        par = t.dtype
+    if not 0.0 <= eps < float('inf'):
+        raise ValueError("eps must be finite and not negative, got %s" % (eps,))
+    return dev, dt, dt if par is None or par == x.dtype else _cabi.F32
+
+
+def _forward(x, weight, bias, eps, want_stats):
+    dev, dt, par = _check(x, weight, bias, eps)
+    flat, rows, d, stride = _cabi.as_rows(x)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if want_stats else None
+    with _cabi.on_device(dev):
+        _cabi.check(_cabi.load_library().b200_layer_norm(
+            flat.data_ptr(), _cabi.ptr(weight), _cabi.ptr(bias), y.data_ptr(), _cabi.ptr(stats), rows, d, stride, dt, par,
+            eps, _cabi.stream_ptr(dev)))
+    return y, flat, weight, stats, par
+
+
+class LayerNormFunc(torch.autograd.Function):
+    """(x, weight or None, bias or None, eps) -> y."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, flat, w, stats, par = _forward(x, weight, bias, eps, True)
+        # (the inputs themselves where the kernel read them, so that a change in place is noticed)
+        ctx.save_for_backward(x if flat.data_ptr() == x.data_ptr() else flat,
+                              weight if w is None or w.data_ptr() == weight.data_ptr() else w, stats)
+        ctx.par, ctx.shape = par, x.shape
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        flat, rows, d, stride = _cabi.as_rows(x)
+        dy, _, _, dy_stride = _cabi.as_rows(dy)
+        dev = flat.device
+        lib = _cabi.load_library()
+        dx = torch.empty(ctx.shape, dtype=flat.dtype, device=dev)
+        dw = torch.empty(d, dtype=weight.dtype, device=dev) if need_w else None
+        db = torch.empty(d, dtype=ctx.bias_dtype, device=dev) if need_b else None
+        scratch, nbytes = None, 0
+        if need_w or need_b:
+            nbytes = lib.b200_layer_norm_scratch_bytes(rows, d)
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        with _cabi.on_device(dev):
+            _cabi.check(lib.b200_layer_norm_backward(
+                flat.data_ptr(), _cabi.ptr(weight), stats.data_ptr(), dy.data_ptr(), dx.data_ptr(), _cabi.ptr(dw),
+                _cabi.ptr(db), _cabi.ptr(scratch), nbytes, rows, d, stride, dy_stride, _cabi.dtype_code(flat), ctx.par,
+                _cabi.stream_ptr(dev)))
+        return dx if need_x else None, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last dimension of x (float32, float16 or bfloat16); weight
+    and bias, either of which may be missing, are float32 or of x's type.  Statistics and sums are float32, results
+    have the type of what they belong to.  Rows may lie apart in memory (one stride between them); the result is
+    contiguous."""
+    eps = float(eps)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return LayerNormFunc.apply(x, weight, bias, eps)
+    return _forward(x, weight, bias, eps, False)[0]
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over rows of `size` elements (the last dimension), as in front of a language model's head:
+
+        >>> norm = LayerNorm(4096).cuda()
+        >>> logits = norm(hidden) @ head.t()        # hidden [..., 4096] float/half/bfloat16
+    """
+
+    def __init__(self, size, eps=1e-5, affine=True, bias=True):
+        super().__init__()
+        self.size, self.eps = int(size), float(eps)
+        self.weight = nn.Parameter(torch.ones(self.size)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(self.size)) if affine and bias else None
+
+    def forward(self, x):
+        if x.dim() < 1 or x.shape[-1] != self.size:
+            raise RuntimeError("rows of %d elements expected, got shape %s" % (self.size, tuple(x.shape)))
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self):
+        return "%d, eps=%g, affine=%s, bias=%s" % (self.size, self.eps, self.weight is not None, self.bias is not None)
