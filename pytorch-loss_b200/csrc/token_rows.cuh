@@ -51,12 +51,13 @@ template <> struct TokenVec<float> {
         return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
                       : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
     }
-    static __device__ __forceinline__ float largest(const uint4 (&v)[kTokenUnroll]) {
-        float m = -INFINITY;
+    static __device__ __forceinline__ float largest(const uint4 &v) {
+        return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+    }
+    template <int COUNT> static __device__ __forceinline__ float largest(const uint4 (&v)[COUNT]) {
+        float m = largest(v[0]);
 #pragma unroll
-        for (int k = 0; k < kTokenUnroll; ++k)
-            m = max_nan(m, max_nan(max_nan(__uint_as_float(v[k].x), __uint_as_float(v[k].y)),
-                                   max_nan(__uint_as_float(v[k].z), __uint_as_float(v[k].w))));
+        for (int k = 1; k < COUNT; ++k) m = max_nan(m, largest(v[k]));
         return m;
     }
     static __device__ __forceinline__ uint4 pack(const float2 (&g)[2]) {
@@ -71,12 +72,17 @@ template <> struct TokenVec<__half> {
     static __device__ __forceinline__ float2 pair(const uint4 &v, int i) {
         return __half22float2(word(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w));
     }
-    static __device__ __forceinline__ float largest(const uint4 (&v)[kTokenUnroll]) {
-        __half2 m = word(kMasked);
+    static __device__ __forceinline__ __half2 largest2(const uint4 &v) {
+        return __hmax2_nan(__hmax2_nan(word(v.x), word(v.y)), __hmax2_nan(word(v.z), word(v.w)));
+    }
+    static __device__ __forceinline__ float largest(const uint4 &v) {
+        const __half2 m = largest2(v);
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    template <int COUNT> static __device__ __forceinline__ float largest(const uint4 (&v)[COUNT]) {
+        __half2 m = largest2(v[0]);
 #pragma unroll
-        for (int k = 0; k < kTokenUnroll; ++k)
-            m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(word(v[k].x), word(v[k].y)),
-                                           __hmax2_nan(word(v[k].z), word(v[k].w))));
+        for (int k = 1; k < COUNT; ++k) m = __hmax2_nan(m, largest2(v[k]));
         return max_nan(__low2float(m), __high2float(m));
     }
     static __device__ __forceinline__ uint4 pack(const float2 (&g)[4]) {
@@ -98,12 +104,17 @@ template <> struct TokenVec<__nv_bfloat16> {
         const unsigned w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
         return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
     }
-    static __device__ __forceinline__ float largest(const uint4 (&v)[kTokenUnroll]) {
-        __nv_bfloat162 m = word(kMasked);
+    static __device__ __forceinline__ __nv_bfloat162 largest2(const uint4 &v) {
+        return __hmax2_nan(__hmax2_nan(word(v.x), word(v.y)), __hmax2_nan(word(v.z), word(v.w)));
+    }
+    static __device__ __forceinline__ float largest(const uint4 &v) {
+        const __nv_bfloat162 m = largest2(v);
+        return max_nan(__low2float(m), __high2float(m));
+    }
+    template <int COUNT> static __device__ __forceinline__ float largest(const uint4 (&v)[COUNT]) {
+        __nv_bfloat162 m = largest2(v[0]);
 #pragma unroll
-        for (int k = 0; k < kTokenUnroll; ++k)
-            m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(word(v[k].x), word(v[k].y)),
-                                           __hmax2_nan(word(v[k].z), word(v[k].w))));
+        for (int k = 1; k < COUNT; ++k) m = __hmax2_nan(m, largest2(v[k]));
         return max_nan(__low2float(m), __high2float(m));
     }
     static __device__ __forceinline__ uint4 pack(const float2 (&g)[4]) {
@@ -117,6 +128,7 @@ template <> struct TokenVec<__nv_bfloat16> {
         return r;
     }
 };
+
 template <typename T> __device__ __forceinline__ uint4 masked_vec() {
     constexpr unsigned w = TokenVec<T>::kMasked;
     return make_uint4(w, w, w, w);
@@ -176,13 +188,14 @@ template <bool ENTROPY> struct RowStat {
         s += e;
         if (ENTROPY) u = fmaf(e, z, u);
     }
-    template <typename T> __device__ __forceinline__ void add(const uint4 (&v)[kTokenUnroll], float c) {
-        const float to = max_nan(m, TokenVec<T>::largest(v));
+    // Some vectors; returns the largest logit among them.
+    template <typename T, int COUNT> __device__ __forceinline__ float add(const uint4 (&v)[COUNT], float c) {
+        const float own = TokenVec<T>::largest(v), to = max_nan(m, own);
         if (!(to <= m)) raise(to, c);
         const pk_t negm = psplat(-reference_of(m)), cc = psplat(c);
         pk_t s2 = psplat(0.f), u2 = psplat(0.f);
 #pragma unroll
-        for (int k = 0; k < kTokenUnroll; ++k) {
+        for (int k = 0; k < COUNT; ++k) {
 #pragma unroll
             for (int i = 0; i < TokenVec<T>::N / 2; ++i) {
                 float2 z = upk2(pmul(padd(pk2(TokenVec<T>::pair(v[k], i)), negm), cc));
@@ -199,6 +212,7 @@ template <bool ENTROPY> struct RowStat {
             const float2 b = upk2(u2);
             u += b.x + b.y;
         }
+        return own;
     }
     // All lanes of a warp: the warp's statistics in every lane.
     __device__ __forceinline__ void join_warp(float c) {
@@ -212,21 +226,39 @@ template <bool ENTROPY> struct RowStat {
 };
 
 // The statistics of a part of a row, the vectors dealt out to G threads in turn; `load(i)` gives the vector that
-// starts at element i.  Every thread returns its own share.
+// starts at element i.  Every thread returns its own share.  `seen(k, m)`: m is the largest logit among the thread's
+// vectors from its k-th on that were just taken in (up to kTokenUnroll of them).
+template <typename T, int G, bool ENTROPY, typename Load, typename Seen>
+__device__ __forceinline__ void scan_part(const T *row, const RowPart &part, int t, float c, RowStat<ENTROPY> &st,
+                                          Load load, Seen seen) {
+    constexpr int N = TokenVec<T>::N, U = kTokenUnroll;
+    const int last_lane = (31 - (t & 31)) * N;              // (a warp takes its steps together)
+    int i = part.body + t * N, k = 0;
+    for (; int64_t(i) + last_lane + (U - 1) * (G * N) < part.body_end; i += U * G * N, k += U) {
+        uint4 v[U];
+#pragma unroll
+        for (int h = 0; h < U; ++h) v[h] = load(i + h * (G * N));
+        seen(k, st.template add<T>(v, c));
+    }
+    // what is left, up to four vectors, some of them not in every lane: all on their way before the first is worked on;
+    // three or four are a batch again, with masked vectors where there are none (one look at the maximum)
+    uint4 v[U];
+#pragma unroll
+    for (int h = 0; h < U; ++h) v[h] = int64_t(i) + h * (G * N) < part.body_end ? load(i + h * (G * N)) : masked_vec<T>();
+    if (__any_sync(0xffffffffu, int64_t(i) + 2 * (G * N) < part.body_end)) {
+        const float most = st.template add<T>(v, c);
+        if (i < part.body_end) seen(k, most);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (int64_t(i) + h * (G * N) < part.body_end) seen(k + h, st.template add<T>(reinterpret_cast<const uint4 (&)[1]>(v[h]), c));
+    }
+    if (t < ragged_count(part)) st.add(to_f32(row[ragged_index(part, t)]), c);
+}
 template <typename T, int G, bool ENTROPY, typename Load>
 __device__ __forceinline__ void scan_part(const T *row, const RowPart &part, int t, float c, RowStat<ENTROPY> &st,
                                           Load load) {
-    constexpr int N = TokenVec<T>::N;
-    for (int i = part.body + t * N; i < part.body_end; i += kTokenUnroll * G * N) {
-        uint4 v[kTokenUnroll];
-#pragma unroll
-        for (int k = 0; k < kTokenUnroll; ++k) {
-            const int64_t at = i + int64_t(k) * (G * N);
-            v[k] = at < part.body_end ? load(int(at)) : masked_vec<T>();
-        }
-        st.template add<T>(v, c);
-    }
-    if (t < ragged_count(part)) st.add(to_f32(row[ragged_index(part, t)]), c);
+    scan_part<T, G>(row, part, t, c, st, load, [](int, float) {});
 }
 
 // ---- host side: launches of clusters of blocks

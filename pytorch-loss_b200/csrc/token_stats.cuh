@@ -51,15 +51,24 @@ template <int G> __device__ __forceinline__ void group_sync() {
 // Candidates that a group of G threads keeps.  32 lanes: their lists are at most 32 long (largest() below).
 template <int G> constexpr int kCandidates = G == 32 ? 256 : 1024;
 
+// A thread's vectors fall into up to kSegments segments of 2^shift vectors (4 at least), whose maxima are kept.
+constexpr int kSegments = 8;
+template <int N, int G> __device__ __forceinline__ int segment_shift(const RowPart &part) {
+    const int per = ((part.body_end - part.body) / N + G - 1) / G;      // vectors of thread 0
+    const int least = (per + kSegments - 1) / kSegments;
+    return least <= 4 ? 2 : 32 - __clz(least - 1);
+}
+
 template <int G, bool TOP> struct TokenShared {
     float m[G / 32], s[G / 32], u[G / 32];
     float joined[3];                                     // this block's share of the row, for the cluster
-    float log2s, row_m;
-    int count;
+    int count, member_count;
     unsigned bound;
-    unsigned short keys[TOP ? G : 1];
+    unsigned short keys[TOP ? G : 1];                    // upper halves of the keys of the threads' maxima ...
+    unsigned short segment[TOP ? kSegments : 1][TOP ? G : 1];   // ... and of those of their segments
+    unsigned short members[TOP ? kSegments * G : 1];     // segments that reach the bound: thread + G * segment
     unsigned hist[TOP ? 256 : 1];
-    unsigned long long cand[TOP ? kCandidates<G> : 1];
+    alignas(16) unsigned long long cand[TOP ? kCandidates<G> : 1];
     unsigned long long best[TOP ? kMaxList : 1];
 };
 
@@ -114,67 +123,124 @@ __device__ __noinline__ unsigned long long exact_bound(const T *row, RowPart par
     return prefix;
 }
 
+// How many of n keys are larger than k.
+__device__ __forceinline__ int larger_keys(const unsigned long long *keys, int n, unsigned long long k) {
+    int a = 0, b = 0;
+    int j = 0;
+#pragma unroll 4
+    for (; j + 1 < n; j += 2) {
+        const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(keys + j);
+        a += two.x > k ? 1 : 0;
+        b += two.y > k ? 1 : 0;
+    }
+    if (j < n) a += keys[j] > k ? 1 : 0;
+    return a + b;
+}
+
+// Of n candidates (0: none) those that reach the K-th largest of their upper 16 bits; returns how many these are.
+template <int G, bool TOP> __device__ __forceinline__ int narrow(int n, int t, int K, TokenShared<G, TOP> &sh) {
+    constexpr int PER = kCandidates<G> / G;
+    if (t < 32) {
+        unsigned bound = 0u;
+#pragma unroll 1
+        for (int bit = 15; bit >= 0; --bit) {
+            const unsigned trial = bound | (1u << bit);
+            unsigned of = 0u;
+            for (int i = t; i < n; i += 32) of += unsigned(sh.cand[i] >> 48) >= trial ? 1u : 0u;
+            if (__reduce_add_sync(0xffffffffu, of) >= unsigned(K)) bound = trial;
+        }
+        if (t == 0) sh.bound = bound;
+    }
+    unsigned long long own[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) own[i] = t + i * G < n ? sh.cand[t + i * G] : 0ull;
+    if (t == 0) sh.count = 0;
+    group_sync<G>();
+    const unsigned bound = sh.bound;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (own[i] && unsigned(own[i] >> 48) >= bound) sh.cand[atomicAdd(&sh.count, 1)] = own[i];
+    group_sync<G>();
+    return sh.count;
+}
+
 // sh.best[0..K) = the K largest keys of the part in order, 0 behind its end.  `m`: the largest logit of each thread.
 //
-// The K-th largest of the threads' maxima is a lower bound of the K-th largest logit, so only the few threads whose
-// maximum reaches it read their logits again (from L2), and what they keep is little more than K.  The bound is taken
-// to the upper 16 bits of the keys: a warp finds it in 16 steps.  The order among the kept is a count of larger keys.
+// The K-th largest of the threads' maxima is a lower bound of the K-th largest logit, so only the few segments whose
+// maximum reaches it are read again (from L2, by all threads at once), and what is kept of them is little more than K.
+// The bound is taken to the upper 16 bits of the keys: a warp finds it in 16 steps.  The order among the kept is a count
+// of larger keys.
 template <typename T, int G, bool TOP, typename Load>
 __device__ __forceinline__ void largest(const T *row, const RowPart &part, int t, float m, int K,
                                         TokenShared<G, TOP> &sh, Load load) {
     constexpr int N = TokenVec<T>::N, PER = G / 32, CAP = kCandidates<G>;
     const unsigned key = value_key(m) >> 16;
     sh.keys[t] = static_cast<unsigned short>(key);
-    if (t == 0) sh.count = 0;
+    if (t == 0) sh.count = sh.member_count = 0;
     group_sync<G>();
     if (t < 32) {
         unsigned k[PER];
 #pragma unroll
         for (int i = 0; i < PER; ++i) k[i] = sh.keys[t + 32 * i];
         unsigned bound = 0u;
-#pragma unroll 1
-        for (int bit = 15; bit >= 0; --bit) {
-            const unsigned trial = bound | (1u << bit);
-            unsigned n = 0u;
+        if (PER > 1 && K <= 24) {                           // (32 maxima say enough)
 #pragma unroll
-            for (int i = 0; i < PER; ++i) n += k[i] >= trial ? 1u : 0u;
-            if (__reduce_add_sync(0xffffffffu, n) >= unsigned(K)) bound = trial;
+            for (int i = 1; i < PER; ++i) k[0] = max(k[0], k[i]);
+#pragma unroll 1
+            for (int bit = 15; bit >= 0; --bit) {
+                const unsigned trial = bound | (1u << bit);
+                if (__popc(__ballot_sync(0xffffffffu, k[0] >= trial)) >= K) bound = trial;
+            }
+        } else {
+#pragma unroll 1
+            for (int bit = 15; bit >= 0; --bit) {
+                const unsigned trial = bound | (1u << bit);
+                unsigned n = 0u;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) n += k[i] >= trial ? 1u : 0u;
+                if (__reduce_add_sync(0xffffffffu, n) >= unsigned(K)) bound = trial;
+            }
         }
         if (t == 0) sh.bound = bound;
     }
     group_sync<G>();
     const unsigned bound = sh.bound;
+    // (the bound as a logit: the smallest value with these upper 16 bits; NaN and "everything" pass every comparison)
+    const float least = bound >= 0xffffu ? INFINITY : bound == 0u ? -INFINITY : key_value(bound << 16);
     auto keep = [&](float x, int j) {
+        if (x < least) return;
         const unsigned long long k = top_key(x, j);
         if (unsigned(k >> 48) >= bound) {
             const int at = atomicAdd(&sh.count, 1);
             if (at < CAP) sh.cand[at] = k;
         }
     };
+    const int shift = segment_shift<N, G>(part);
     if (key >= bound) {
-        for (int i = part.body + t * N; i < part.body_end; i += kTokenUnroll * G * N) {
-            uint4 v[kTokenUnroll];
-#pragma unroll
-            for (int k = 0; k < kTokenUnroll; ++k) {
-                const int64_t at = i + int64_t(k) * (G * N);
-                if (at < part.body_end) v[k] = load(int(at));
-            }
-#pragma unroll
-            for (int k = 0; k < kTokenUnroll; ++k) {
-                const int64_t at = i + int64_t(k) * (G * N);
-                if (at < part.body_end) {
-#pragma unroll
-                    for (int h = 0; h < N / 2; ++h) {
-                        const float2 x = TokenVec<T>::pair(v[k], h);
-                        keep(x.x, int(at) + 2 * h);
-                        keep(x.y, int(at) + 2 * h + 1);
-                    }
-                }
-            }
-        }
+        const int per = ((part.body_end - part.body) / N - t + G - 1) / G;          // this thread's vectors
+        for (int i = 0; i << shift < per; ++i)
+            if (sh.segment[i][t] >= bound) sh.members[atomicAdd(&sh.member_count, 1)] = static_cast<unsigned short>(t + G * i);
         if (t < ragged_count(part)) {
             const int j = ragged_index(part, t);
             keep(to_f32(row[j]), j);
+        }
+    }
+    group_sync<G>();
+    // the vectors of these segments, dealt out to all threads: `lanes` threads to each
+    const int members = sh.member_count, lane_shift = min(shift, 5), lanes = 1 << lane_shift;
+    for (int i = t >> lane_shift; i < members; i += G >> lane_shift) {
+        const int owner = sh.members[i] % G, first = sh.members[i] / G << shift;
+        for (int k = t & (lanes - 1); k < 1 << shift; k += lanes) {
+            const int64_t at = part.body + (owner + int64_t(first + k) * G) * N;
+            if (at >= part.body_end) break;
+            const uint4 v = load(int(at));
+            if (TokenVec<T>::largest(v) < least) continue;
+#pragma unroll
+            for (int h = 0; h < N / 2; ++h) {
+                const float2 x = TokenVec<T>::pair(v, h);
+                keep(x.x, int(at) + 2 * h);
+                keep(x.y, int(at) + 2 * h + 1);
+            }
         }
     }
     group_sync<G>();
@@ -189,23 +255,17 @@ __device__ __forceinline__ void largest(const T *row, const RowPart &part, int t
         }
         group_sync<G>();
         n = sh.count;
+    } else if (n > 2 * K + 32) {
+        n = narrow<G>(n, t, K, sh);                         // (short rows and long lists: the threads' maxima say little)
     }
     for (int i = t; i < K; i += G)
         if (i >= n) sh.best[i] = 0ull;
     for (int i = t; i < n; i += G) {
         const unsigned long long k = sh.cand[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += sh.cand[j] > k ? 1 : 0;
+        const int rank = larger_keys(sh.cand, n, k);
         if (rank < K) sh.best[rank] = k;
     }
     group_sync<G>();
-}
-
-__device__ __forceinline__ void write_alternative(const TokenParams &p, int64_t row, int i, unsigned long long key,
-                                                  float m, float log2s, bool nothing) {
-    const float x = key_value(unsigned(key >> 32));
-    p.top_logprobs[row * p.K + i] = nothing ? -INFINITY : log_prob(x, m, p.inv_t, log2s);
-    p.top_tokens[row * p.K + i] = int64_t(~unsigned(key));
 }
 
 // G threads to a row (32: eight rows to a block), or the G threads of each of `parts` blocks.
@@ -258,7 +318,22 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
     auto load = [row](int i) { return ld_stream16<uint4>(row + i); };
     RowStat<ENTROPY> st;
     st.init();
-    scan_part<T, G, ENTROPY>(row, part, t, p.c, st, load);
+    if constexpr (TOP) {
+        const int shift = segment_shift<TokenVec<T>::N, G>(part);
+        int current = 0;
+        float most = -INFINITY;
+        scan_part<T, G>(row, part, t, p.c, st, load, [&](int k, float m) {
+            if (k >> shift != current) {
+                sh.segment[current][t] = static_cast<unsigned short>(value_key(most) >> 16);
+                current = k >> shift;
+                most = -INFINITY;
+            }
+            most = max_nan(most, m);
+        });
+        sh.segment[current][t] = static_cast<unsigned short>(value_key(most) >> 16);
+    } else {
+        scan_part<T, G>(row, part, t, p.c, st, load);
+    }
     const float own_max = st.m;
     st.join_warp(p.c);
     if (G > 32) {
@@ -268,16 +343,19 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
             if (ENTROPY) sh.u[t >> 5] = st.u;
         }
         __syncthreads();
-        st.init();
-        if (lane < WARPS) {
-            st.m = sh.m[lane];
-            st.s = sh.s[lane];
-            if (ENTROPY) st.u = sh.u[lane];
+        if (t < 32) {                                       // the block's statistics: the first warp's business
+            st.init();
+            if (lane < WARPS) {
+                st.m = sh.m[lane];
+                st.s = sh.s[lane];
+                if (ENTROPY) st.u = sh.u[lane];
+            }
+            st.join_warp(p.c);
         }
-        st.join_warp(p.c);
     }
     if constexpr (TOP) largest<T, G, TOP>(row, part, t, own_max, p.K, sh, load);
 
+    int found = TOP ? p.K : 0;
     if (G > 32 && parts > 1) {
         namespace cg = cooperative_groups;
         cg::cluster_group cluster = cg::this_cluster();
@@ -288,33 +366,46 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
         }
         cluster.sync();
         if (rank == 0) {
-            st.init();
-            if (lane < parts) {
-                const float *other = cluster.map_shared_rank(&sh.joined[0], lane);
-                st.m = other[0];
-                st.s = other[1];
-                if (ENTROPY) st.u = other[2];
-            }
-            st.join_warp(p.c);
-            if constexpr (TOP) {
-                for (int i = t; i < parts * p.K; i += G)
-                    sh.cand[i] = cluster.map_shared_rank(&sh.best[0], i / p.K)[i % p.K];
-                __syncthreads();
-                for (int i = t; i < parts * p.K; i += G) {
-                    const unsigned long long k = sh.cand[i];
-                    int place = 0;
-                    for (int j = 0; j < parts * p.K; ++j) place += sh.cand[j] > k ? 1 : 0;
-                    if (k != 0ull && place < p.K)
-                        write_alternative(p, r, place, k, reference_of(st.m), log2f(st.s), st.s == 0.f);
+            if (t < 32) {
+                st.init();
+                if (lane < parts) {
+                    const float *other = cluster.map_shared_rank(&sh.joined[0], lane);
+                    st.m = other[0];
+                    st.s = other[1];
+                    if (ENTROPY) st.u = other[2];
                 }
+                st.join_warp(p.c);
+            }
+            if constexpr (TOP) {
+                found = parts * p.K;                        // (0 where a part has fewer logits)
+                for (int i = t; i < found; i += G)
+                    sh.cand[i] = cluster.map_shared_rank(&sh.best[0], i / p.K)[i % p.K];
             }
         }
         cluster.sync();                                     // (nobody leaves while its memory is read)
         if (rank != 0) return;
-    } else if constexpr (TOP) {
-        for (int i = t; i < p.K; i += G)
-            write_alternative(p, r, i, sh.best[i], reference_of(st.m), log2f(st.s), st.s == 0.f);
+        if constexpr (TOP) {
+            if (found > 2 * p.K + 32) found = narrow<G, TOP>(found, t, p.K, sh);
+        }
     }
+    if constexpr (TOP) {
+        // the first warp's statistics for all
+        if (t == 0) {
+            sh.joined[0] = reference_of(st.m);
+            sh.joined[1] = st.s == 0.f ? INFINITY : log2f(st.s);    // (a row of -inf: every log probability is -inf)
+        }
+        group_sync<G>();
+        const float m = sh.joined[0], log2s = sh.joined[1];
+        for (int i = t; i < found; i += G) {
+            const unsigned long long k = parts > 1 ? sh.cand[i] : sh.best[i];
+            const int place = parts > 1 ? larger_keys(sh.cand, found, k) : i;
+            if (k == 0ull || place >= p.K) continue;
+            const float x = key_value(unsigned(k >> 32));
+            p.top_logprobs[r * p.K + place] = log2s == INFINITY ? -INFINITY : log_prob(x, m, p.inv_t, log2s);
+            p.top_tokens[r * p.K + place] = int64_t(~unsigned(k));
+        }
+    }
+    if (t >= 32) return;
 
     const float m = reference_of(st.m), log2s = log2f(st.s);
     const bool nothing = st.s == 0.f;                       // a row of -inf
@@ -326,7 +417,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
             p.entropy[r] = nothing ? 0.f : max_nan(kTokenLn2 * (log2s - mean), 0.f);
             if (p.stats) p.stats[r] = make_float4(m, nothing ? 0.f : 1.f / st.s, mean, log2s);
         }
-    } else if (t < 32) {
+    } else {
         // sum of w (log w - log p) over the list; `given` holds the sum of w log w
         float part_loss = 0.f;
         for (int i = lane; i < p.K; i += 32) {
@@ -484,9 +575,8 @@ __global__ void __launch_bounds__(256) token_grad_kernel(const TokenGradParams p
 
 // ---- launches
 
-// How many threads share a row and over how many blocks it is split.  Rows of up to 4 KB are a warp's (no barrier;
-// lists of alternatives up to 32).  Longer rows are a block's; with few rows they are split over the blocks of a
-// cluster, as long as all of them run at once and every thread still has a vector.
+// Over how many blocks of a cluster a row is split: with few rows, as long as all blocks run at once and every thread
+// still has a vector.
 inline int row_parts(int64_t rows, int64_t V, int dtype) {
     const int64_t vectors = row_vectors(V, dtype), room = int64_t(sm_count()) * 8;
     int parts = 1;
@@ -494,15 +584,26 @@ inline int row_parts(int64_t rows, int64_t V, int dtype) {
     return parts;
 }
 
+// How many threads share a row.  What a row costs besides its elements (joins, barriers, finding the alternatives) is
+// paid per thread, so few threads are better -- as long as there are rows enough to fill the SMs several times over,
+// and a list of alternatives is short against the number of threads.  Measured, us at 32 / 128 / 256 threads:
+//   [32768, 4000] bfloat16 (8 KB)     log probabilities 58 / 82 / 120    with 20 alternatives 121 / 176 / 269
+//   [16384, 8192] float32 (32 KB)     84 / 80 / 87                       161 / 120 / 155
+//   [16384, 32768] bfloat16 (64 KB)   173 / 168 / 174                    792 / 224 / 259
+//   [2047, 100003] float16 (200 KB)   -- / 80 / 72                       -- / 101 / 89     (one wave of 128 threads)
+//   128 alternatives of [16384, 32768]: -- / 1409 / 433
 template <typename T, int MODE, bool TOP> int launch_stats(const TokenParams &prm, int dtype, cudaStream_t stream) {
     TokenParams p = prm;
     const char *what = "token statistics kernel launch";
     if (p.rows == 0) return B200_OK;
-    if (p.V * int64_t(sizeof(T)) <= 4096 && !(TOP && p.K > 32)) {
-        p.parts = 1;
+    const int64_t bytes = p.V * int64_t(sizeof(T)), sms = sm_count();
+    const bool shortlist = !TOP || p.K <= 32;
+    p.parts = 1;
+    if (shortlist && (bytes <= 4096 || (p.rows >= 32 * sms && bytes <= (TOP ? 16384 : 32768))))
         return launch_cluster(token_stats_kernel<T, 32, MODE, TOP>, (p.rows + 7) / 8, 256, 0, 1, false, stream, what, p);
-    }
     p.parts = row_parts(p.rows, p.V, dtype);
+    if (p.parts == 1 && shortlist && (p.rows >= 32 * sms || bytes <= 131072))
+        return launch_cluster(token_stats_kernel<T, 128, MODE, TOP>, p.rows, 128, 0, 1, false, stream, what, p);
     return launch_cluster(token_stats_kernel<T, 256, MODE, TOP>, p.rows * p.parts, 256, 0, p.parts, false, stream, what,
                           p);
 }

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kStepThreads) distill_step_kernel(const StepPa
     RowStat<false> st;
     st.init();
     auto load = [&](int i) { return held[(i - part.body) / N]; };
-    if (arrived) scan_part<T, kStepThreads, false>(row, part, t, p.c, st, load);
+    if (arrived) scan_part<T, kStepThreads>(row, part, t, p.c, st, load);
     else st.m = __int_as_float(0x7fc00000);                 // (a copy that never came shows as NaN)
     st.join_warp(p.c);
     if (lane == 0) {

@@ -30,12 +30,12 @@ __all__ += ["TaylorSoftmaxV3", "LogTaylorSoftmaxV3", "TaylorCrossEntropyLossV3",
 from .pc_softmax import PCSoftmaxCrossEntropyV2, PCSoftmaxCrossEntropyFunction
 
 __all__ += ["PCSoftmaxCrossEntropyV2", "PCSoftmaxCrossEntropyFunction"]
-from .token_logprobs import TokenLogProbs, TokenLogProbsFunc, token_logprobs
+from .logprobs import TokenLogProbs, TokenLogProbsFunc, token_logprobs
 
 __all__ += ["TokenLogProbs", "TokenLogProbsFunc", "token_logprobs"]
 from .top_distill import TopTokenDistillLoss, TopTokenDistillFunc
 
 __all__ += ["TopTokenDistillLoss", "TopTokenDistillFunc"]
-from .layer_norm import LayerNorm, LayerNormFunc, layer_norm
+from .norm import LayerNorm, LayerNormFunc, layer_norm
 
 __all__ += ["LayerNorm", "LayerNormFunc", "layer_norm"]

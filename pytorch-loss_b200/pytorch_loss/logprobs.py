@@ -5,7 +5,6 @@ forward, one more with the gradient's write backward; nothing of the vocabulary'
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _cabi
 
@@ -41,14 +40,15 @@ def _forward(dev, logits, tokens, top_k, temperature, ignore_index, want_stats):
     dt = _cabi.dtype_code(flat)
     shape = tokens.shape
     tokens = tokens.contiguous()
-    logprobs = torch.empty(shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+    # (allocations by *_like and new_empty: half the host time of torch.empty with a device)
+    logprobs = tokens.new_empty(shape, dtype=torch.float32)
+    entropy = torch.empty_like(logprobs)
     top_lp = top_tok = stats = None
     if top_k:
-        top_lp = torch.empty(shape + (top_k,), dtype=torch.float32, device=dev)
-        top_tok = torch.empty(shape + (top_k,), dtype=torch.int64, device=dev)
+        top_lp = logprobs.new_empty(shape + (top_k,))
+        top_tok = tokens.new_empty(shape + (top_k,))
     if want_stats:
-        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+        stats = logprobs.new_empty((rows, 4))
     lib = _cabi.load_library()
     with _cabi.on_device(dev):
         _cabi.check(lib.b200_token_logprobs(
@@ -71,14 +71,14 @@ class TokenLogProbsFunc(torch.autograd.Function):
             # (the input itself where the kernel read it, so that a change in place is noticed)
             shared = flat.data_ptr() == logits.data_ptr()
             ctx.save_for_backward(logits if shared else flat, tok, stats)
-            ctx.shape, ctx.temperature, ctx.ignore_index = logits.shape, temperature, ignore_index
+            ctx.info = logits.shape, temperature, ignore_index
         ctx.set_materialize_grads(False)
         if top_k:
             ctx.mark_non_differentiable(top_lp, top_tok)
         return logprobs, entropy, top_lp, top_tok
 
     @staticmethod
-    @once_differentiable
+    @_cabi.once_differentiable
     def backward(ctx, d_logprobs, d_entropy, _top_logprobs, _top_tokens):
         if d_logprobs is None and d_entropy is None:
             return None, None, None, None, None
@@ -89,11 +89,11 @@ class TokenLogProbsFunc(torch.autograd.Function):
             d_logprobs = d_logprobs.contiguous()
         if d_entropy is not None:
             d_entropy = d_entropy.contiguous()
-        grad = torch.empty(ctx.shape, dtype=flat.dtype, device=dev)
+        grad = flat.new_empty(ctx.info[0])
         with _cabi.on_device(dev):
             _cabi.check(_cabi.load_library().b200_token_logprobs_backward(
                 flat.data_ptr(), tokens.data_ptr(), stats.data_ptr(), _cabi.ptr(d_logprobs), _cabi.ptr(d_entropy),
-                grad.data_ptr(), rows, v, stride, _cabi.dtype_code(flat), ctx.temperature, ctx.ignore_index,
+                grad.data_ptr(), rows, v, stride, _cabi.dtype_code(flat), ctx.info[1], ctx.info[2],
                 _cabi.stream_ptr(dev)))
         return grad, None, None, None, None
 
