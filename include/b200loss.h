@@ -447,7 +447,8 @@ int b200_token_logprobs_backward(const void *logits, const int64_t *tokens, cons
  *       scratch: what the forward call of the same inputs left
  *   step    : out and the final gradient (mean: divided by the number of counted rows) from ONE read of
  *       the logits; b200_top_distill_step_path: 1 when the layout has it (float32 / bfloat16, gradient
- *       rows at the logits' place within 16 bytes, rows of up to 1.6 MB).  float16 has none: there the
+ *       rows at the logits' place within 16 bytes, rows of more than 4 KB and up to 320 KB; others are as
+ *       fast in two passes).  float16 has none: there the
  *       upstream gradient (loss scaling) has to come in before the one rounding.  Backward of the step is
  *       b200_rescale_gradient.
  * scratch: b200_top_distill_scratch_bytes(rows, K) bytes, 16-byte aligned, contents irrelevant. */

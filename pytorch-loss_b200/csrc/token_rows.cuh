@@ -8,8 +8,8 @@
 // rises (once per 4 vectors at most), threads, warps and the blocks of a cluster are joined afterwards.
 //
 // The difference x_j - m is formed before the scaling, so rows of the type's lowest value (a mask that left nothing)
-// stay finite, and z_j is held at -200 or more (2^-200 is 0 here), so that a masked logit (-inf) adds 0 * -200 and
-// not 0 * inf to u.  Maxima hand NaN on: a NaN logit gives NaN results, never a hidden one.  A row of -inf alone has
+// stay finite.  Where z_j itself enters a sum it is held at -200 or more (2^-200 is 0 here), so that a masked logit
+// (-inf) adds 0 * -200 and not 0 * inf to u.  Maxima hand NaN on: a NaN logit gives NaN results, never a hidden one.  A row of -inf alone has
 // s = 0; each kernel says what it returns there.
 //
 // A row starts wherever its tensor puts it: the elements in front of the first 16-byte boundary and behind the last
@@ -136,22 +136,38 @@ template <typename T> __device__ __forceinline__ uint4 masked_vec() {
 
 // ---- which part of a row a block reads
 
-// Elements [first, last) of a row; [body, body_end) of them are whole 16-byte vectors at 16-byte addresses.  Part
-// `rank` of `parts` of the row; the ragged ends belong to the first and the last part.
+// Elements [first, last) of a row; [body, body_end) of them are whole 16-byte vectors at 16-byte addresses.  The ragged
+// ends belong to the first and the last part.
 struct RowPart {
     int first, body, body_end, last;
 };
-template <typename T>
-__device__ __forceinline__ RowPart row_part(const T *row, int V, int rank, int parts) {
-    constexpr int N = TokenVec<T>::N;
+template <typename T> __device__ __forceinline__ int ragged_head(const T *row, int V) {
     const int off = int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    const int head = min(V, off ? N - off : 0);
+    return min(V, off ? TokenVec<T>::N - off : 0);
+}
+// Part `rank` of 2^shift parts of a row (no division: it would cost a thread as much as 20 elements).
+template <typename T>
+__device__ __forceinline__ RowPart row_part(const T *row, int V, int rank, int shift) {
+    constexpr int N = TokenVec<T>::N;
+    const int head = ragged_head(row, V);
     const int64_t nvec = (V - head) / N;
     RowPart r;
-    r.body = head + int(nvec * rank / parts) * N;
-    r.body_end = head + int(nvec * (rank + 1) / parts) * N;
+    r.body = head + int(nvec * rank >> shift) * N;
+    r.body_end = head + int(nvec * (rank + 1) >> shift) * N;
     r.first = rank == 0 ? 0 : r.body;
-    r.last = rank == parts - 1 ? V : r.body_end;
+    r.last = rank + 1 == 1 << shift ? V : r.body_end;
+    return r;
+}
+// Chunk `index` of `chunks` chunks of `vectors` vectors (the last one: what is left).
+template <typename T>
+__device__ __forceinline__ RowPart row_chunk(const T *row, int V, int index, int chunks, int vectors) {
+    constexpr int N = TokenVec<T>::N;
+    const int head = ragged_head(row, V), nvec = (V - head) / N;
+    RowPart r;
+    r.body = head + min(nvec, index * vectors) * N;
+    r.body_end = head + min(nvec, (index + 1) * vectors) * N;
+    r.first = index == 0 ? 0 : r.body;
+    r.last = index == chunks - 1 ? V : r.body_end;
     return r;
 }
 // The i-th element of a part that no vector covers (i < ragged_count), as an index into the row.
@@ -199,8 +215,10 @@ template <bool ENTROPY> struct RowStat {
 #pragma unroll
             for (int i = 0; i < TokenVec<T>::N / 2; ++i) {
                 float2 z = upk2(pmul(padd(pk2(TokenVec<T>::pair(v[k], i)), negm), cc));
-                z.x = max_nan(z.x, kTokenFloor);
-                z.y = max_nan(z.y, kTokenFloor);
+                if (ENTROPY) {
+                    z.x = max_nan(z.x, kTokenFloor);
+                    z.y = max_nan(z.y, kTokenFloor);
+                }
                 const pk_t zz = pk2(z), e = pex2(zz);
                 s2 = padd(s2, e);
                 if (ENTROPY) u2 = pfma(e, zz, u2);
@@ -227,15 +245,17 @@ template <bool ENTROPY> struct RowStat {
 
 // The statistics of a part of a row, the vectors dealt out to G threads in turn; `load(i)` gives the vector that
 // starts at element i.  Every thread returns its own share.  `seen(k, m)`: m is the largest logit among the thread's
-// vectors from its k-th on that were just taken in (up to kTokenUnroll of them).
-template <typename T, int G, bool ENTROPY, typename Load, typename Seen>
+// vectors from its k-th on that were just taken in (up to kTokenUnroll of them).  `ready(k)` is called before the
+// thread's vectors from its k-th on, up to kTokenUnroll of them, are loaded (k a multiple of that).
+template <typename T, int G, bool ENTROPY, typename Load, typename Seen, typename Ready>
 __device__ __forceinline__ void scan_part(const T *row, const RowPart &part, int t, float c, RowStat<ENTROPY> &st,
-                                          Load load, Seen seen) {
+                                          Load load, Seen seen, Ready ready) {
     constexpr int N = TokenVec<T>::N, U = kTokenUnroll;
     const int last_lane = (31 - (t & 31)) * N;              // (a warp takes its steps together)
     int i = part.body + t * N, k = 0;
     for (; int64_t(i) + last_lane + (U - 1) * (G * N) < part.body_end; i += U * G * N, k += U) {
         uint4 v[U];
+        ready(k);
 #pragma unroll
         for (int h = 0; h < U; ++h) v[h] = load(i + h * (G * N));
         seen(k, st.template add<T>(v, c));
@@ -243,6 +263,7 @@ __device__ __forceinline__ void scan_part(const T *row, const RowPart &part, int
     // what is left, up to four vectors, some of them not in every lane: all on their way before the first is worked on;
     // three or four are a batch again, with masked vectors where there are none (one look at the maximum)
     uint4 v[U];
+    if (i < part.body_end) ready(k);
 #pragma unroll
     for (int h = 0; h < U; ++h) v[h] = int64_t(i) + h * (G * N) < part.body_end ? load(i + h * (G * N)) : masked_vec<T>();
     if (__any_sync(0xffffffffu, int64_t(i) + 2 * (G * N) < part.body_end)) {
@@ -258,7 +279,7 @@ __device__ __forceinline__ void scan_part(const T *row, const RowPart &part, int
 template <typename T, int G, bool ENTROPY, typename Load>
 __device__ __forceinline__ void scan_part(const T *row, const RowPart &part, int t, float c, RowStat<ENTROPY> &st,
                                           Load load) {
-    scan_part<T, G>(row, part, t, c, st, load, [](int, float) {});
+    scan_part<T, G>(row, part, t, c, st, load, [](int, float) {}, [](int) {});
 }
 
 // ---- host side: launches of clusters of blocks

@@ -23,7 +23,7 @@ struct TokenParams {
     float4 *stats;              // {m, 1 / s, u / s, log2 s} for the gradient (may be null)
     float *top_logprobs;
     int64_t *top_tokens;
-    int parts;                  // blocks of a cluster that share a row
+    int part_shift;             // 2^part_shift blocks of a cluster share a row
 };
 
 // ---- alternatives
@@ -278,9 +278,9 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
     __shared__ TokenShared<G, TOP> shared[GROUPS];
     const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x, lane = threadIdx.x & 31;
     TokenShared<G, TOP> &sh = shared[G == 32 ? threadIdx.x >> 5 : 0];
-    const int parts = G == 32 ? 1 : p.parts;
-    const int rank = G == 32 ? 0 : int(blockIdx.x % unsigned(parts));
-    const int64_t r = G == 32 ? int64_t(blockIdx.x) * GROUPS + (threadIdx.x >> 5) : int64_t(blockIdx.x / unsigned(parts));
+    const int parts = 1 << (G == 32 ? 0 : p.part_shift);
+    const int rank = G == 32 ? 0 : int(blockIdx.x) & (parts - 1);
+    const int64_t r = G == 32 ? int64_t(blockIdx.x) * GROUPS + (threadIdx.x >> 5) : int64_t(blockIdx.x >> p.part_shift);
     if (r >= p.rows) return;
     const T *row = static_cast<const T *>(p.x) + r * p.stride;
 
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
         }
     }
 
-    const RowPart part = row_part(row, p.V, rank, parts);
+    const RowPart part = row_part(row, p.V, rank, G == 32 ? 0 : p.part_shift);
     auto load = [row](int i) { return ld_stream16<uint4>(row + i); };
     RowStat<ENTROPY> st;
     st.init();
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
                 most = -INFINITY;
             }
             most = max_nan(most, m);
-        });
+        }, [](int) {});
         sh.segment[current][t] = static_cast<unsigned short>(value_key(most) >> 16);
     } else {
         scan_part<T, G>(row, part, t, p.c, st, load);
@@ -435,6 +435,76 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
     }
 }
 
+// A thread's entries of a row's list that lie in a part of the row: weight (0: none), token and logit.  Loaded under the
+// row's own loads, so that the accesses one after the other cost nothing behind them.
+template <typename T, int G> struct ListShare {
+    static constexpr int N = kMaxList > G ? kMaxList / G : 1;
+    float w[N], x[N];
+    int64_t id[N];
+    // What the list says ...
+    __device__ __forceinline__ void load(const int64_t *ids, const float *weight, int K, int t) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool there = t + i * G < K;
+            w[i] = there ? weight[t + i * G] : 0.f;
+            id[i] = there ? ids[t + i * G] : -1;
+            x[i] = 0.f;
+        }
+    }
+    // ... and the logits it asks for: weight 0 for what is not in this part.
+    __device__ __forceinline__ void fetch(const RowPart &part, const T *row) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (w[i] > 0.f && id[i] >= part.first && id[i] < part.last) x[i] = to_f32(row[id[i]]);
+            else w[i] = 0.f;
+        }
+    }
+};
+
+// Which entries of a row's list each thread meets among the elements it writes: the thread that owns an element is
+// handed its entry, so that the element leaves complete (a second, 2-byte store to lines on their way to memory cost
+// the gradient kernel 20 %: [16384, 32768] bfloat16 with lists of 20 391 against @@ us).
+template <int G> struct ListChain {
+    int head[G];
+    int next[kMaxList], at[kMaxList];
+    float w[kMaxList];
+};
+// All threads of the group; returns this thread's first entry (-1: none).
+template <typename T, int G>
+__device__ __forceinline__ int deal_list(const ListShare<T, G> &list, const RowPart &part, int t, ListChain<G> &chain) {
+    chain.head[t] = -1;
+    group_sync<G>();
+#pragma unroll
+    for (int k = 0; k < list.N; ++k) {
+        if (list.w[k] > 0.f && list.id[k] >= part.first && list.id[k] < part.last) {
+            const int i = t + k * G, j = int(list.id[k]);
+            const int owner = j < part.body       ? j - part.first
+                              : j < part.body_end ? (j - part.body) / TokenVec<T>::N % G
+                                                  : part.body - part.first + j - part.body_end;
+            chain.at[i] = j;
+            chain.w[i] = list.w[k];
+            chain.next[i] = atomicExch(&chain.head[owner], i);
+        }
+    }
+    group_sync<G>();
+    return chain.head[t];
+}
+// Adds scale * w to what the list asks for among the 2 * PAIRS elements from `first` on.
+template <int G, int PAIRS>
+__device__ __forceinline__ void add_entries(float2 (&d)[PAIRS], int first, int entry, const ListChain<G> &chain, float scale) {
+    for (; entry >= 0; entry = chain.next[entry]) {
+        const int at = chain.at[entry] - first;
+        const float w = chain.w[entry];
+        if (unsigned(at) < unsigned(2 * PAIRS)) {
+#pragma unroll
+            for (int h = 0; h < PAIRS; ++h) {
+                if (at == 2 * h) d[h].x = fmaf(scale, w, d[h].x);
+                if (at == 2 * h + 1) d[h].y = fmaf(scale, w, d[h].y);
+            }
+        }
+    }
+}
+
 // ---- gradient from the statistics
 // kTokens: g_j = e_j (A + B z_j) + dl [j = token] / T,  A = -(dl - dh ln2 u / s) / (s T),  B = -dh ln2 / (s T)
 // kList:   g_j = scale (p_j - w_j) / T
@@ -465,111 +535,108 @@ __global__ void __launch_bounds__(256) token_grad_kernel(const TokenGradParams p
     constexpr int N = TokenVec<T>::N;
     constexpr int GROUPS = 256 / G;
     const int t = threadIdx.x % G;
-    const int64_t unit = int64_t(blockIdx.x) * GROUPS + threadIdx.x / G;
-    const int64_t r = unit / p.chunks;
-    const int chunk = int(unit % p.chunks);
+    const unsigned unit = blockIdx.x * GROUPS + threadIdx.x / G;
+    const int64_t r = G == 32 ? unit : unit / unsigned(p.chunks);
+    const int chunk = G == 32 ? 0 : int(unit % unsigned(p.chunks));
     if (r >= p.rows) return;
     const T *x = static_cast<const T *>(p.x) + r * p.stride;
     T *g = static_cast<T *>(p.grad) + r * int64_t(p.V);
 
-    float A = 0.f, B = 0.f, at_token = 0.f, m = 0.f;
+    // everything that hangs on nothing first
+    const int64_t id = MODE == kTokens ? p.ids[r] : 0;
+    const float base = MODE == kList ? p.base[r] : 0.f;
+    const float4 st = p.stats[r];                           // (not written for rows that are not asked for: not used then)
+    float dl = p.d_out ? p.d_out[r * p.d_out_step] : 0.f;
+    const float dh = MODE == kTokens && p.d_entropy ? p.d_entropy[r] : 0.f;
+    ListShare<T, G> list;
+    if (MODE == kList) list.load(p.ids + r * p.K, p.weight + r * p.K, p.K, t);
+
+    float A = 0.f, B = 0.f, at_token = 0.f;
     int token = -1;
-    bool zero = false;
-    if (MODE == kTokens) {
-        const int64_t id = p.ids[r];
-        zero = id == p.ignore;
-        if (!zero) {
-            const float4 st = p.stats[r];
-            float dl = p.d_out ? p.d_out[r * p.d_out_step] : 0.f;
-            const float dh = p.d_entropy ? p.d_entropy[r] : 0.f;
+    const float m = st.x;
+    bool zero = MODE == kTokens ? id == p.ignore : base == INFINITY;
+    if (!zero) {
+        if (MODE == kTokens) {
             const bool bad = id < 0 || id >= p.V;
             if (bad) dl = __int_as_float(0x7fc00000);
-            m = st.x;
             B = -dh * kTokenLn2 * st.y * p.inv_t;
             A = -(dl - dh * kTokenLn2 * st.z) * st.y * p.inv_t;
             token = bad ? -1 : int(id);
             at_token = dl * p.inv_t;
             zero = st.y == 0.f && !bad;
-        }
-    } else {
-        const float base = p.base[r];
-        zero = base == INFINITY;
-        if (!zero) {
-            const float4 st = p.stats[r];
-            float scale = p.d_out[r * p.d_out_step] * p.inv_t;
+        } else {
+            float scale = dl * p.inv_t;
             if (p.count) scale = float(double(scale) / *p.count);
             if (base != base) scale = base;
-            m = st.x;
             A = scale * st.y;
             at_token = -scale;
             zero = st.y == 0.f;
         }
     }
 
-    const RowPart part = row_part(static_cast<const T *>(g), p.V, chunk, p.chunks);
+    const RowPart part = row_chunk(static_cast<const T *>(g), p.V, chunk, p.chunks, G * kTokenUnroll);
     const pk_t negm = psplat(-m), cc = psplat(p.c), aa = psplat(A), bb = psplat(B);
     auto one = [&](float v) {                               // without what a given token adds
         const float z = max_nan((v - m) * p.c, kTokenFloor), e = ex2f(z);
         return e * fmaf(B, z, A);
     };
-    for (int i = part.body + t * N; i < part.body_end; i += kTokenUnroll * G * N) {
-        uint4 v[kTokenUnroll];
+    // (a chunk is one step: its vectors are all on their way before the first is worked on)
+    const int i = part.body + t * N;
+    uint4 v[kTokenUnroll];
 #pragma unroll
-        for (int k = 0; k < kTokenUnroll; ++k) {
-            const int64_t at = i + int64_t(k) * (G * N);
-            v[k] = make_uint4(0u, 0u, 0u, 0u);
-            if (!zero && at < part.body_end) {
-                if (ALIGNED) {
-                    v[k] = ld_stream16<uint4>(x + at);
-                } else {
-                    T e[N];
+    for (int k = 0; k < kTokenUnroll; ++k) {
+        const int64_t at = i + int64_t(k) * (G * N);
+        v[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (!zero && at < part.body_end) {
+            if (ALIGNED) {
+                v[k] = ld_stream16<uint4>(x + at);
+            } else {
+                T e[N];
 #pragma unroll
-                    for (int h = 0; h < N; ++h) e[h] = x[at + h];
-                    memcpy(&v[k], e, 16);
-                }
+                for (int h = 0; h < N; ++h) e[h] = x[at + h];
+                memcpy(&v[k], e, 16);
             }
         }
+    }
+    __shared__ ListChain<G> chains[MODE == kList ? GROUPS : 1];
+    ListChain<G> &chain = chains[MODE == kList ? threadIdx.x / G : 0];
+    const int entry = MODE == kList && !zero ? deal_list(list, part, t, chain) : -1;
 #pragma unroll
-        for (int k = 0; k < kTokenUnroll; ++k) {
-            const int64_t at = i + int64_t(k) * (G * N);
-            if (at >= part.body_end) break;
-            if (!zero) {
-                float2 d[N / 2];
+    for (int k = 0; k < kTokenUnroll; ++k) {
+        const int64_t at = i + int64_t(k) * (G * N);
+        if (at >= part.body_end) break;
+        if (!zero) {
+            float2 d[N / 2];
 #pragma unroll
-                for (int h = 0; h < N / 2; ++h) {
-                    float2 z = upk2(pmul(padd(pk2(TokenVec<T>::pair(v[k], h)), negm), cc));
+            for (int h = 0; h < N / 2; ++h) {
+                float2 z = upk2(pmul(padd(pk2(TokenVec<T>::pair(v[k], h)), negm), cc));
+                if (MODE == kTokens) {
                     z.x = max_nan(z.x, kTokenFloor);
                     z.y = max_nan(z.y, kTokenFloor);
-                    const pk_t zz = pk2(z);
-                    const pk_t e = pex2(zz);
-                    d[h] = upk2(MODE == kTokens ? pmul(e, pfma(bb, zz, aa)) : pmul(e, aa));
                 }
-                if (MODE == kTokens && unsigned(token - int(at)) < unsigned(N)) {
-                    const int w = token - int(at);
-#pragma unroll
-                    for (int h = 0; h < N / 2; ++h) {
-                        if (w == 2 * h) d[h].x += at_token;
-                        if (w == 2 * h + 1) d[h].y += at_token;
-                    }
-                }
-                v[k] = TokenVec<T>::pack(d);
+                const pk_t zz = pk2(z);
+                const pk_t e = pex2(zz);
+                d[h] = upk2(MODE == kTokens ? pmul(e, pfma(bb, zz, aa)) : pmul(e, aa));
             }
-            st_stream16(g + at, v[k]);
+            if (MODE == kTokens && unsigned(token - int(at)) < unsigned(N)) {
+                const int w = token - int(at);
+#pragma unroll
+                for (int h = 0; h < N / 2; ++h) {
+                    if (w == 2 * h) d[h].x += at_token;
+                    if (w == 2 * h + 1) d[h].y += at_token;
+                }
+            }
+            if (MODE == kList) add_entries(d, int(at), entry, chain, at_token);
+            v[k] = TokenVec<T>::pack(d);
         }
+        st_stream16(g + at, v[k]);
     }
     if (t < ragged_count(part)) {
         const int j = ragged_index(part, t);
-        const float d = zero ? 0.f : one(to_f32(x[j]));
-        g[j] = from_f32<T>(MODE == kTokens && !zero && j == token ? d + at_token : d);
-    }
-    if (MODE == kList && !zero) {
-        group_sync<G>();                                    // (what the list changes has been written)
-        for (int i = t; i < p.K; i += G) {
-            const float w = p.weight[r * p.K + i];
-            const int64_t j = p.ids[r * p.K + i];
-            if (w > 0.f && j >= part.first && j < part.last)
-                g[j] = from_f32<T>(fmaf(at_token, w, one(to_f32(x[j]))));
-        }
+        float2 d[1] = {make_float2(zero ? 0.f : one(to_f32(x[j])), 0.f)};
+        if (MODE == kTokens && !zero && j == token) d[0].x += at_token;
+        if (MODE == kList) add_entries(d, j, entry, chain, at_token);
+        g[j] = from_f32<T>(d[0].x);
     }
 }
 
@@ -577,11 +644,11 @@ __global__ void __launch_bounds__(256) token_grad_kernel(const TokenGradParams p
 
 // Over how many blocks of a cluster a row is split: with few rows, as long as all blocks run at once and every thread
 // still has a vector.
-inline int row_parts(int64_t rows, int64_t V, int dtype) {
+inline int row_part_shift(int64_t rows, int64_t V, int dtype) {
     const int64_t vectors = row_vectors(V, dtype), room = int64_t(sm_count()) * 8;
-    int parts = 1;
-    while (parts < kMaxCluster && rows * parts * 2 <= room && vectors / (parts * 2) >= 256) parts *= 2;
-    return parts;
+    int shift = 0;
+    while (2 << shift <= kMaxCluster && rows << (shift + 1) <= room && vectors >> (shift + 1) >= 256) ++shift;
+    return shift;
 }
 
 // How many threads share a row.  What a row costs besides its elements (joins, barriers, finding the alternatives) is
@@ -598,13 +665,13 @@ template <typename T, int MODE, bool TOP> int launch_stats(const TokenParams &pr
     if (p.rows == 0) return B200_OK;
     const int64_t bytes = p.V * int64_t(sizeof(T)), sms = sm_count();
     const bool shortlist = !TOP || p.K <= 32;
-    p.parts = 1;
+    p.part_shift = 0;
     if (shortlist && (bytes <= 4096 || (p.rows >= 32 * sms && bytes <= (TOP ? 16384 : 32768))))
         return launch_cluster(token_stats_kernel<T, 32, MODE, TOP>, (p.rows + 7) / 8, 256, 0, 1, false, stream, what, p);
-    p.parts = row_parts(p.rows, p.V, dtype);
-    if (p.parts == 1 && shortlist && (p.rows >= 32 * sms || bytes <= 131072))
+    p.part_shift = row_part_shift(p.rows, p.V, dtype);
+    if (p.part_shift == 0 && shortlist && (p.rows >= 32 * sms || bytes <= 131072))
         return launch_cluster(token_stats_kernel<T, 128, MODE, TOP>, p.rows, 128, 0, 1, false, stream, what, p);
-    return launch_cluster(token_stats_kernel<T, 256, MODE, TOP>, p.rows * p.parts, 256, 0, p.parts, false, stream, what,
+    return launch_cluster(token_stats_kernel<T, 256, MODE, TOP>, p.rows << p.part_shift, 256, 0, 1 << p.part_shift, false, stream, what,
                           p);
 }
 

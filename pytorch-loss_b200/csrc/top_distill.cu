@@ -5,18 +5,17 @@
 // any mass is not read, costs nothing and counts for nothing in a mean.
 //
 // distill_lists_kernel turns the lists into weights once (one warp per row), the other kernels take these.  The
-// training step ('mean' / 'sum') holds the row in shared memory -- split over the blocks of a cluster where it is
-// longer than one block's share -- and reads the logits once; without it the statistics kernel and the gradient
+// training step ('mean' / 'sum') reads the logits from memory once; without it the statistics kernel and the gradient
 // kernel of token_stats.cuh read them once each.
 #include "token_stats.cuh"
 
 namespace b200 {
 namespace {
 
+constexpr int kListWarps = 16;              // rows of a block of the list kernel
 constexpr int kListSlots = 512;             // blocks of the list kernel, at most: each counts its rows
-constexpr int kStepThreads = 512;
-constexpr size_t kStepShare = 64 * 1024;    // bytes of a row per block where eight blocks suffice
-constexpr size_t kStepMost = 200 * 1024;    // beyond: two passes
+constexpr size_t kStepHeld = 72 * 1024;     // longest row that a block holds: three blocks on an SM
+constexpr int kStepPieces = 16;             // of 8 KB (128 threads) or 16 KB (256)
 
 // Scratch: the blocks' row counts, then per row statistics, sum of w log w, loss and weights.
 struct DistillScratch {
@@ -36,15 +35,17 @@ inline DistillScratch carve(void *scratch, int64_t rows) {
     return d;
 }
 
-__global__ void __launch_bounds__(256) distill_lists_kernel(const int64_t *tokens, const float *q, float *weight,
+__global__ void __launch_bounds__(32 * kListWarps) distill_lists_kernel(const int64_t *tokens, const float *q, float *weight,
                                                             float *base, int *counts, int64_t rows, int K, int V) {
-    __shared__ int ids[8][kMaxList];
-    __shared__ float ws[8][kMaxList];
-    __shared__ int valid_rows[8];
+    static_assert(kMaxList == 128, "four entries a lane");
+    __shared__ __align__(16) int ids[kListWarps][kMaxList];
+    __shared__ float ws[kListWarps][kMaxList];
+    __shared__ int valid_rows[kListWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int valid = 0;
-    for (int64_t r = int64_t(blockIdx.x) * 8 + warp; r < rows; r += int64_t(gridDim.x) * 8) {
-        float x[kMaxList / 32];
+    for (int64_t r = int64_t(blockIdx.x) * kListWarps + warp; r < rows; r += int64_t(gridDim.x) * kListWarps) {
+        float x[kMaxList / 32], w[kMaxList / 32];
+        int own[kMaxList / 32];
         float best = -INFINITY;
         bool bad = false;
 #pragma unroll
@@ -57,7 +58,8 @@ __global__ void __launch_bounds__(256) distill_lists_kernel(const int64_t *token
                 if (id >= 0) x[e] = q[r * K + i];
                 bad = bad || id >= V;
             }
-            ids[warp][i] = id >= 0 && id < V ? int(id) : -1;
+            own[e] = id >= 0 && id < V ? int(id) : -1;
+            ids[warp][i] = own[e];
             best = max_nan(best, x[e]);
         }
 #pragma unroll
@@ -66,32 +68,55 @@ __global__ void __launch_bounds__(256) distill_lists_kernel(const int64_t *token
         const bool nothing = best == -INFINITY && !bad;
         float total = 0.f;
 #pragma unroll
-        for (int e = 0; e < kMaxList / 32; ++e) total += x[e] == -INFINITY ? 0.f : expf(x[e] - best);
+        for (int e = 0; e < kMaxList / 32; ++e) {
+            if (32 * e >= K) break;
+            x[e] = x[e] == -INFINITY ? -INFINITY : x[e] - best;
+            w[e] = x[e] == -INFINITY ? 0.f : expf(x[e]);
+            total += w[e];
+        }
         total = warp_sum(total);
         const float log_total = logf(total);
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < kMaxList / 32; ++e) {
-            const float lw = x[e] - best - log_total;
-            const float w = x[e] == -INFINITY ? 0.f : expf(x[e] - best) / total;
-            if (w > 0.f || w != w) sum += w * lw;
-            ws[warp][lane + 32 * e] = ids[warp][lane + 32 * e] < 0 ? 0.f : w;
+            if (32 * e >= K) break;
+            w[e] /= total;
+            if (w[e] > 0.f || w[e] != w[e]) sum += w[e] * (x[e] - log_total);
+            ws[warp][lane + 32 * e] = own[e] < 0 ? 0.f : w[e];
         }
         sum = warp_sum(sum);
         __syncwarp();
-        // entries with the same token: the first one carries the weight of all
+        // the same token twice?  Rare: only looked for here
+        int twins = 0;
+        for (int j = 0; j < K; j += 4) {
+            const int4 four = *reinterpret_cast<const int4 *>(&ids[warp][j]);
+#pragma unroll
+            for (int e = 0; e < kMaxList / 32; ++e) {
+                if (32 * e >= K) break;
+                const int id = own[e];
+                twins += (four.x == id) + (four.y == id) + (four.z == id) + (four.w == id);
+            }
+        }
+        // (every entry meets itself; tokens that do not exist meet each other, which only costs the longer way)
+#pragma unroll
+        for (int e = 0; e < kMaxList / 32; ++e) twins -= lane + 32 * e < K ? 1 : 0;
+        const bool merge = __any_sync(0xffffffffu, twins > 0);
         for (int e = 0; e * 32 < K; ++e) {
             const int i = lane + 32 * e;
             if (i >= K) break;
-            const int id = ids[warp][i];
-            float w = 0.f;
-            bool first = id >= 0;
-            for (int j = 0; j < K; ++j)
-                if (ids[warp][j] == id) {
-                    first = first && j >= i;
-                    w += ws[warp][j];
-                }
-            weight[r * K + i] = first ? w : 0.f;
+            float sum_w = ws[warp][i];
+            if (merge) {                                    // the first of such entries carries the weight of all
+                const int id = ids[warp][i];
+                bool first = id >= 0;
+                sum_w = 0.f;
+                for (int j = 0; j < K; ++j)
+                    if (ids[warp][j] == id) {
+                        first = first && j >= i;
+                        sum_w += ws[warp][j];
+                    }
+                if (!first) sum_w = 0.f;
+            }
+            weight[r * K + i] = sum_w;
         }
         if (lane == 0) base[r] = bad ? __int_as_float(0x7fc00000) : nothing ? INFINITY : sum;
         valid += nothing ? 0 : 1;
@@ -101,11 +126,11 @@ __global__ void __launch_bounds__(256) distill_lists_kernel(const int64_t *token
     __syncthreads();
     if (threadIdx.x == 0) {
         int n = 0;
-        for (int w = 0; w < 8; ++w) n += valid_rows[w];
+        for (int w = 0; w < kListWarps; ++w) n += valid_rows[w];
         counts[blockIdx.x] = n;
     }
     if (blockIdx.x == 0)
-        for (int i = int(gridDim.x) + int(threadIdx.x); i < kListSlots; i += 256) counts[i] = 0;
+        for (int i = int(gridDim.x) + int(threadIdx.x); i < kListSlots; i += 32 * kListWarps) counts[i] = 0;
 }
 
 // record = {sum of the losses, number of rows that have one, mean, sum}: one block, so the order is always the same.
@@ -129,7 +154,7 @@ struct StepParams {
     const void *x;
     void *grad;
     int64_t stride, rows;
-    int V, K, parts;
+    int V, K, part_shift;       // 2^part_shift blocks of a cluster share a row
     float c, inv_t;
     const int64_t *ids;
     const float *weight, *base;
@@ -137,52 +162,65 @@ struct StepParams {
     float *losses;
 };
 
-// One row per cluster of `parts` blocks; each block's part of it is copied to shared memory once (bulk copy), read
-// twice there (statistics, gradient), and the gradient leaves as 16-byte stores.
+// One row per block (HELD: copied to shared memory once, in pieces, and read twice there) or per cluster of up to two
+// blocks (read twice, the second time from L2).  The gradient leaves as 16-byte stores, and what the list changes is
+// written once more behind them.
 // Bound: HBM, 2 x the logits' bytes; two exponentials an element and the joins between the blocks come next.
-template <typename T>
-__global__ void __launch_bounds__(kStepThreads) distill_step_kernel(const StepParams p) {
+template <typename T, int THREADS, bool HELD>
+__global__ void __launch_bounds__(THREADS) distill_step_kernel(const StepParams p) {
     namespace cg = cooperative_groups;
-    constexpr int N = TokenVec<T>::N, WARPS = kStepThreads / 32;
+    constexpr int N = TokenVec<T>::N, WARPS = THREADS / 32;
     extern __shared__ __align__(16) uint4 held[];
-    __shared__ uint64_t full;
-    __shared__ float wm[WARPS], wsum[WARPS], joined[2];
+    __shared__ uint64_t full[kStepPieces];
+    __shared__ float wm[WARPS], wsum[WARPS], wloss[WARPS], joined[3];
     __shared__ int wcount[WARPS];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int rank = int(blockIdx.x % unsigned(p.parts));
-    const int64_t r = int64_t(blockIdx.x / unsigned(p.parts));
+    const int parts = 1 << p.part_shift, rank = int(blockIdx.x) & (parts - 1);
+    const int64_t r = int64_t(blockIdx.x >> p.part_shift);
     const T *row = static_cast<const T *>(p.x) + r * p.stride;
     T *g = static_cast<T *>(p.grad) + r * int64_t(p.V);
-    const RowPart part = row_part(row, p.V, rank, p.parts);
+    const RowPart part = row_part(row, p.V, rank, p.part_shift);
     const float base = p.base[r];
+    ListShare<T, THREADS> list;
+    list.load(p.ids + r * p.K, p.weight + r * p.K, p.K, t);
+    int count = 0;
+    if (p.counts && t < kListSlots / 4) {
+        const int4 four = reinterpret_cast<const int4 *>(p.counts)[t];
+        count = (four.x + four.y) + (four.z + four.w);
+    }
     if (base == INFINITY) {                                 // (all blocks of the cluster)
-        for (int i = part.body + t * N; i < part.body_end; i += kStepThreads * N)
+        for (int i = part.body + t * N; i < part.body_end; i += THREADS * N)
             st_stream16(g + i, make_uint4(0u, 0u, 0u, 0u));
         if (t < ragged_count(part)) g[ragged_index(part, t)] = from_f32<T>(0.f);
         if (rank == 0 && t == 0) p.losses[r] = 0.f;
         return;
     }
-    const int n = part.body_end - part.body;
-    if (t == 0) {
-        mbar_init(&full, 1);
-        fence_mbar_init();
-        if (n > 0) {
-            const uint32_t bytes = uint32_t(n) * uint32_t(sizeof(T));
-            mbar_expect_tx(&full, bytes);
-            bulk_load_1d(held, row + part.body, bytes, &full);
+    // (pieces of as many vectors as a step of all threads takes: work begins with the first)
+    constexpr int PIECE = kTokenUnroll * THREADS * N;
+    if (HELD) {
+        if (t == 0) {
+            for (int i = 0; i < kStepPieces; ++i) mbar_init(&full[i], 1);
+            fence_mbar_init();
+            for (int i = 0; part.body + i * PIECE < part.body_end; ++i) {
+                const int n = min(PIECE, part.body_end - part.body - i * PIECE);
+                mbar_expect_tx(&full[i], uint32_t(n) * uint32_t(sizeof(T)));
+                bulk_load_1d(held + i * (PIECE / N), row + part.body + i * PIECE, uint32_t(n) * uint32_t(sizeof(T)), &full[i]);
+            }
         }
+        __syncthreads();
     }
-    __syncthreads();
-    int count = p.counts && t < kListSlots ? p.counts[t] : 0;
-    count = __reduce_add_sync(0xffffffffu, count);
-    const bool arrived = n == 0 || mbar_wait_bounded(&full, 0, nullptr);
+    list.fetch(part, row);
 
     RowStat<false> st;
     st.init();
-    auto load = [&](int i) { return held[(i - part.body) / N]; };
-    if (arrived) scan_part<T, kStepThreads>(row, part, t, p.c, st, load);
-    else st.m = __int_as_float(0x7fc00000);                 // (a copy that never came shows as NaN)
+    bool arrived = true;
+    auto load = [&](int i) { return HELD ? held[(i - part.body) / N] : *reinterpret_cast<const uint4 *>(row + i); };
+    scan_part<T, THREADS>(row, part, t, p.c, st, load, [](int, float) {}, [&](int k) {
+        if (HELD && arrived) arrived = mbar_wait_bounded(&full[k / kTokenUnroll], 0, nullptr);
+    });
+    if (!arrived) st.m = __int_as_float(0x7fc00000);        // (a copy that never came shows as NaN)
     st.join_warp(p.c);
+    count = __reduce_add_sync(0xffffffffu, count);
     if (lane == 0) {
         wm[warp] = st.m;
         wsum[warp] = st.s;
@@ -199,39 +237,36 @@ __global__ void __launch_bounds__(kStepThreads) distill_step_kernel(const StepPa
     st.join_warp(p.c);
     count = __reduce_add_sync(0xffffffffu, count);
     cg::cluster_group cluster = cg::this_cluster();
-    if (p.parts > 1) {
+    if (parts > 1) {
         if (t == 0) {
             joined[0] = st.m;
             joined[1] = st.s;
         }
         cluster.sync();
         st.init();
-        if (lane < p.parts) {
+        if (lane < parts) {
             const float *other = cluster.map_shared_rank(&joined[0], lane);
             st.m = other[0];
             st.s = other[1];
         }
         st.join_warp(p.c);
-        cluster.barrier_arrive();                           // (this block has read what it needs)
     }
 
-    const float m = reference_of(st.m);
+    const float m = reference_of(st.m), log2s = log2f(st.s);
     const bool nothing = st.s == 0.f;
     float scale = p.inv_t;
     if (p.counts) scale /= float(count);
     if (base != base) scale = base;
     const float A = nothing ? 0.f : scale / st.s;
-    auto one = [&](float v) { return ex2f(max_nan((v - m) * p.c, kTokenFloor)) * A; };
+    auto one = [&](float v) { return ex2f((v - m) * p.c) * A; };
     const pk_t negm = psplat(-m), cc = psplat(p.c), aa = psplat(A);
-    for (int i = part.body + t * N; i < part.body_end; i += kStepThreads * N) {
+#pragma unroll 4
+    for (int i = part.body + t * N; i < part.body_end; i += THREADS * N) {
         const uint4 v = load(i);
         float2 d[N / 2];
 #pragma unroll
         for (int h = 0; h < N / 2; ++h) {
-            float2 z = upk2(pmul(padd(pk2(TokenVec<T>::pair(v, h)), negm), cc));
-            z.x = max_nan(z.x, kTokenFloor);
-            z.y = max_nan(z.y, kTokenFloor);
-            d[h] = upk2(pmul(pex2(pk2(z)), aa));
+            d[h] = upk2(pmul(pex2(pmul(padd(pk2(TokenVec<T>::pair(v, h)), negm), cc)), aa));
         }
         st_stream16(g + i, TokenVec<T>::pack(d));
     }
@@ -239,46 +274,76 @@ __global__ void __launch_bounds__(kStepThreads) distill_step_kernel(const StepPa
         const int j = ragged_index(part, t);
         g[j] = from_f32<T>(one(to_f32(row[j])));
     }
-    __syncthreads();                                        // (what the list changes has been written)
+    // each block's part of the loss: sum over its part of the list
     float loss = 0.f;
-    for (int i = t; i < p.K; i += kStepThreads) {
-        const float w = p.weight[r * p.K + i];
-        if (w > 0.f) {
-            const int64_t j = p.ids[r * p.K + i];
-            const float x = to_f32(row[j]);
-            if (j >= part.first && j < part.last && !nothing) g[j] = from_f32<T>(fmaf(-scale, w, one(x)));
-            loss = fmaf(-w, nothing ? -INFINITY : log_prob(x, m, p.inv_t, log2f(st.s)), loss);
+#pragma unroll
+    for (int i = 0; i < list.N; ++i)
+        if (list.w[i] > 0.f) loss = fmaf(-list.w[i], nothing ? -INFINITY : log_prob(list.x[i], m, p.inv_t, log2s), loss);
+    loss = warp_sum(loss);
+    if (lane == 0) wloss[warp] = loss;
+    __syncthreads();                                        // (what the list changes has been written, too)
+#pragma unroll
+    for (int i = 0; i < list.N; ++i)
+        if (list.w[i] > 0.f && !nothing) g[list.id[i]] = from_f32<T>(fmaf(-scale, list.w[i], one(list.x[i])));
+    if (t == 0) {
+        loss = 0.f;
+        for (int i = 0; i < WARPS; ++i) loss += wloss[i];
+        joined[2] = loss;
+    }
+    if (parts > 1) {
+        cluster.sync();
+        if (rank == 0 && t == 0) {
+            for (int i = 1; i < parts; ++i) loss += cluster.map_shared_rank(&joined[0], i)[2];
         }
+        if (rank == 0 && t == 0) p.losses[r] = base + loss;
+        cluster.sync();                                     // (nobody leaves while its memory is read)
+    } else if (t == 0) {
+        p.losses[r] = base + loss;
     }
-    if (rank == 0) {                                        // (the list lies in the first four warps)
-        loss = warp_sum(loss);
-        if (lane == 0) wm[warp] = loss;
-        __syncthreads();
-        if (t == 0) p.losses[r] = base + (wm[0] + wm[1]) + (wm[2] + wm[3]);
-    }
-    if (p.parts > 1) cluster.barrier_wait();                // (nobody leaves while its memory is read)
 }
 
-inline int step_parts(int64_t V, int dtype) {
-    const size_t bytes = size_t(V) * dtype_size(dtype);
-    int parts = 1;
-    while (parts < kMaxCluster && bytes > kStepShare * parts) parts *= 2;
-    return bytes <= kStepMost * parts ? parts : 0;
+// How a step treats a row.  Measured (us, lists of 20; two passes: statistics, then gradient):
+//   [16384, 4096] bfloat16 (8 KB)     held by 128 threads 79, 256 110           two passes 103
+//   [16384, 16384] bfloat16 (32 KB)   held by 128 193, 256 190, 512 262         270
+//   [16384, 32768] bfloat16 (64 KB)   held by 128 424, 256 374, 512 387         505    from L2, 512 threads: 406
+//   [8192, 24000] float32 (96 KB)     held by 256 322                           360    from L2: 272
+//   [8192, 65536] bfloat16 (128 KB)   held by two blocks 436                    493    from L2: 412, two blocks 479
+//   [3000, 50001] float32 (200 KB)    275                                       281    from L2: 299, two blocks 255
+//   [4096, 131072] bfloat16 (256 KB)  513                                       483    from L2: 519, two blocks 437
+//   [2048, 131072] float32 (512 KB)   503                                       482    from L2: 532, two blocks 529
+// From L2 works while the rows under way fit there (three blocks of 512 threads an SM: 57 MB at 128 KB); blocks of a
+// cluster wait for each other's place on the chip.
+enum StepWay { kNoStep, kHeld128, kHeld256, kFromL2, kFromL2Pair };
+inline StepWay step_way(int64_t V, int dtype) {
+    const int64_t bytes = V * int64_t(dtype_size(dtype));
+    return bytes <= 4096                ? kNoStep
+           : bytes <= 16 * 1024         ? kHeld128
+           : bytes <= int64_t(kStepHeld) ? kHeld256
+           : bytes <= 160 * 1024        ? kFromL2
+           : bytes <= 320 * 1024        ? kFromL2Pair
+                                        : kNoStep;
 }
 
-template <typename T> int launch_step(const StepParams &p, cudaStream_t stream) {
-    const size_t vectors = (size_t(p.V) * sizeof(T) / 16 + p.parts - 1) / p.parts;
-    const size_t bytes = vectors * 16 + 16;
-    if (const int rc = set_smem(distill_step_kernel<T>, bytes)) return rc;
-    return launch_cluster(distill_step_kernel<T>, p.rows * p.parts, kStepThreads, bytes, p.parts, false, stream,
-                          "distillation step kernel launch", p);
+template <typename T, int THREADS> int launch_held(const StepParams &p, const char *what, cudaStream_t stream) {
+    const size_t bytes = size_t(p.V) * sizeof(T) / 16 * 16;
+    if (const int rc = set_smem(distill_step_kernel<T, THREADS, true>, bytes)) return rc;
+    return launch_cluster(distill_step_kernel<T, THREADS, true>, p.rows, THREADS, bytes, 1, false, stream, what, p);
+}
+template <typename T> int launch_step(StepParams p, int dtype, cudaStream_t stream) {
+    const char *what = "distillation step kernel launch";
+    const StepWay way = step_way(p.V, dtype);
+    if (way == kHeld128) return launch_held<T, 128>(p, what, stream);
+    if (way == kHeld256) return launch_held<T, 256>(p, what, stream);
+    p.part_shift = way == kFromL2Pair ? 1 : 0;
+    return launch_cluster(distill_step_kernel<T, 512, false>, p.rows << p.part_shift, 512, 0, 1 << p.part_shift, false,
+                          stream, what, p);
 }
 
 int launch_lists(const int64_t *tokens, const float *q, const DistillScratch &d, int64_t rows, int K, int V,
                  cudaStream_t stream) {
-    int64_t grid = (rows + 7) / 8;
+    int64_t grid = (rows + kListWarps - 1) / kListWarps;
     grid = grid < 1 ? 1 : grid > kListSlots ? kListSlots : grid;
-    distill_lists_kernel<<<unsigned(grid), 256, 0, stream>>>(tokens, q, d.weight, d.base, d.counts, rows, K, V);
+    distill_lists_kernel<<<unsigned(grid), 32 * kListWarps, 0, stream>>>(tokens, q, d.weight, d.base, d.counts, rows, K, V);
     return launch_status("distillation list kernel launch");
 }
 
@@ -385,7 +450,7 @@ extern "C" int b200_top_distill_step_path(const void *logits, const void *grad_l
         return 0;
     if (((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(grad_logits)) & 15) != 0) return 0;
     if (rows > 1 && ((stride - V) * int64_t(dtype_size(dtype))) % 16 != 0) return 0;
-    return step_parts(V, dtype) > 0;
+    return step_way(V, dtype) != kNoStep;
 }
 
 extern "C" int b200_top_distill_step(const void *logits, const int64_t *top_tokens, const float *top_logprobs,
@@ -409,7 +474,6 @@ extern "C" int b200_top_distill_step(const void *logits, const int64_t *top_toke
     p.rows = rows;
     p.V = int(V);
     p.K = K;
-    p.parts = step_parts(V, dtype);
     p.c = float(1.4426950408889634 / double(temperature));
     p.inv_t = 1.f / temperature;
     p.ids = top_tokens;
@@ -417,7 +481,7 @@ extern "C" int b200_top_distill_step(const void *logits, const int64_t *top_toke
     p.base = d.base;
     p.counts = mean ? d.counts : nullptr;
     p.losses = d.losses;
-    const int rc = dtype == B200_F32 ? launch_step<float>(p, s) : launch_step<__nv_bfloat16>(p, s);
+    const int rc = dtype == B200_F32 ? launch_step<float>(p, dtype, s) : launch_step<__nv_bfloat16>(p, dtype, s);
     if (rc) return rc;
     distill_finish_kernel<<<1, 1024, 0, s>>>(d.losses, d.counts, rows, static_cast<ReduceRecord *>(out));
     return launch_status("distillation sum kernel launch");

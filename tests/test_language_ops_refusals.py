@@ -71,7 +71,8 @@ def test_which_layouts_have_the_one_pass_step(lib):
     assert q(4, 32768, 32768, F32) == 1 and q(4, 131072, 131072, BF16) == 1
     assert q(4, 50001, 50001, F32) == 1                          # odd rows: gradient rows lie like the logits'
     assert q(4, 50001, 50048, F32) == 0 and q(1, 50001, 50048, F32) == 1
-    assert q(4, 400000, 400000, F32) == 1 and q(4, 420000, 420000, F32) == 0      # 8 x 200 KB
+    assert q(4, 81920, 81920, F32) == 1 and q(4, 81921, 81921, F32) == 0          # rows of more than 4 to 320 KB
+    assert q(4, 1025, 1025, F32) == 1 and q(4, 1024, 1024, F32) == 0 and q(4, 2048, 2048, BF16) == 0
     assert q(4, 32768, 32768, F16) == 0 and q(0, 32768, 32768, F32) == 0
     assert q(4, 32768, 32768, F32, ctypes.c_void_p(0x7f0000001004)) == 0
 
