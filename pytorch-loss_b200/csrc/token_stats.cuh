@@ -307,6 +307,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const To
         bad = token < 0 || token >= p.V;
         if (rank == 0 && t == 0 && !bad) given = to_f32(row[token]);
     } else {
+        pdl_wait();                                         // (the lists' kernel)
         given = p.base[r];
         if (given == INFINITY) {
             if (rank == 0 && t == 0) p.out[r] = 0.f;
@@ -667,11 +668,11 @@ template <typename T, int MODE, bool TOP> int launch_stats(const TokenParams &pr
     const bool shortlist = !TOP || p.K <= 32;
     p.part_shift = 0;
     if (shortlist && (bytes <= 4096 || (p.rows >= 32 * sms && bytes <= (TOP ? 16384 : 32768))))
-        return launch_cluster(token_stats_kernel<T, 32, MODE, TOP>, (p.rows + 7) / 8, 256, 0, 1, false, stream, what, p);
+        return launch_cluster(token_stats_kernel<T, 32, MODE, TOP>, (p.rows + 7) / 8, 256, 0, 1, MODE == kList, stream, what, p);
     p.part_shift = row_part_shift(p.rows, p.V, dtype);
     if (p.part_shift == 0 && shortlist && (p.rows >= 32 * sms || bytes <= 131072))
-        return launch_cluster(token_stats_kernel<T, 128, MODE, TOP>, p.rows, 128, 0, 1, false, stream, what, p);
-    return launch_cluster(token_stats_kernel<T, 256, MODE, TOP>, p.rows << p.part_shift, 256, 0, 1 << p.part_shift, false, stream, what,
+        return launch_cluster(token_stats_kernel<T, 128, MODE, TOP>, p.rows, 128, 0, 1, MODE == kList, stream, what, p);
+    return launch_cluster(token_stats_kernel<T, 256, MODE, TOP>, p.rows << p.part_shift, 256, 0, 1 << p.part_shift, MODE == kList, stream, what,
                           p);
 }
 

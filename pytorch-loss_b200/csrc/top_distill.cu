@@ -42,6 +42,7 @@ __global__ void __launch_bounds__(32 * kListWarps) distill_lists_kernel(const in
     __shared__ float ws[kListWarps][kMaxList];
     __shared__ int valid_rows[kListWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();                                // (the kernel behind takes its place on the SMs meanwhile)
     int valid = 0;
     for (int64_t r = int64_t(blockIdx.x) * kListWarps + warp; r < rows; r += int64_t(gridDim.x) * kListWarps) {
         float x[kMaxList / 32], w[kMaxList / 32];
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(32 * kListWarps) distill_lists_kernel(const in
 __global__ void __launch_bounds__(1024) distill_finish_kernel(const float *losses, const int *counts, int64_t rows,
                                                               ReduceRecord *out) {
     __shared__ double sh[64];
+    pdl_wait();
     double sum = 0.0, count = threadIdx.x < kListSlots ? double(counts[threadIdx.x]) : 0.0;
     for (int64_t i = threadIdx.x; i < rows; i += 1024) sum += double(losses[i]);
     block_sum2(sum, count, sh);
@@ -180,6 +182,7 @@ __global__ void __launch_bounds__(THREADS) distill_step_kernel(const StepParams 
     const T *row = static_cast<const T *>(p.x) + r * p.stride;
     T *g = static_cast<T *>(p.grad) + r * int64_t(p.V);
     const RowPart part = row_part(row, p.V, rank, p.part_shift);
+    pdl_wait();                                             // (the lists' kernel)
     const float base = p.base[r];
     ListShare<T, THREADS> list;
     list.load(p.ids + r * p.K, p.weight + r * p.K, p.K, t);
@@ -327,7 +330,7 @@ inline StepWay step_way(int64_t V, int dtype) {
 template <typename T, int THREADS> int launch_held(const StepParams &p, const char *what, cudaStream_t stream) {
     const size_t bytes = size_t(p.V) * sizeof(T) / 16 * 16;
     if (const int rc = set_smem(distill_step_kernel<T, THREADS, true>, bytes)) return rc;
-    return launch_cluster(distill_step_kernel<T, THREADS, true>, p.rows, THREADS, bytes, 1, false, stream, what, p);
+    return launch_cluster(distill_step_kernel<T, THREADS, true>, p.rows, THREADS, bytes, 1, true, stream, what, p);
 }
 template <typename T> int launch_step(StepParams p, int dtype, cudaStream_t stream) {
     const char *what = "distillation step kernel launch";
@@ -335,8 +338,13 @@ template <typename T> int launch_step(StepParams p, int dtype, cudaStream_t stre
     if (way == kHeld128) return launch_held<T, 128>(p, what, stream);
     if (way == kHeld256) return launch_held<T, 256>(p, what, stream);
     p.part_shift = way == kFromL2Pair ? 1 : 0;
-    return launch_cluster(distill_step_kernel<T, 512, false>, p.rows << p.part_shift, 512, 0, 1 << p.part_shift, false,
+    return launch_cluster(distill_step_kernel<T, 512, false>, p.rows << p.part_shift, 512, 0, 1 << p.part_shift, true,
                           stream, what, p);
+}
+
+int launch_finish(const float *losses, const int *counts, int64_t rows, void *out, cudaStream_t stream) {
+    return launch_cluster(distill_finish_kernel, 1, 1024, 0, 1, true, stream, "distillation sum kernel launch", losses, counts,
+                          rows, static_cast<ReduceRecord *>(out));
 }
 
 int launch_lists(const int64_t *tokens, const float *q, const DistillScratch &d, int64_t rows, int K, int V,
@@ -405,8 +413,7 @@ extern "C" int b200_top_distill_forward(const void *logits, const int64_t *top_t
                    : dtype == B200_F16 ? launch_stats<__half, kList, false>(p, dtype, s)
                                        : launch_stats<__nv_bfloat16, kList, false>(p, dtype, s);
     if (rc || !out) return rc;
-    distill_finish_kernel<<<1, 1024, 0, s>>>(p.out, d.counts, rows, static_cast<ReduceRecord *>(out));
-    return launch_status("distillation sum kernel launch");
+    return launch_finish(p.out, d.counts, rows, out, s);
 }
 
 extern "C" int b200_top_distill_backward(const void *logits, const int64_t *top_tokens, const void *scratch,
@@ -483,6 +490,5 @@ extern "C" int b200_top_distill_step(const void *logits, const int64_t *top_toke
     p.losses = d.losses;
     const int rc = dtype == B200_F32 ? launch_step<float>(p, dtype, s) : launch_step<__nv_bfloat16>(p, dtype, s);
     if (rc) return rc;
-    distill_finish_kernel<<<1, 1024, 0, s>>>(d.losses, d.counts, rows, static_cast<ReduceRecord *>(out));
-    return launch_status("distillation sum kernel launch");
+    return launch_finish(d.losses, d.counts, rows, out, s);
 }

@@ -65,14 +65,15 @@ def _step(logits, top_tokens, top_logprobs, temperature, reduction):
     if dt == _cabi.F16 or rows == 0:
         return None
     grad = flat.new_empty(logits.shape)
-    if not lib.b200_top_distill_step_path(flat.data_ptr(), grad.data_ptr(), rows, v, stride, dt):
-        return None
     scratch = _scratch(lib, q, rows, k)
     rec = q.new_empty(8)
     with _cabi.on_device(dev):
-        _cabi.check(lib.b200_top_distill_step(
+        code = lib.b200_top_distill_step(
             flat.data_ptr(), tok.data_ptr(), q.data_ptr(), grad.data_ptr(), rec.data_ptr(), scratch.data_ptr(),
-            4 * scratch.numel(), rows, v, stride, dt, k, temperature, int(reduction == 'mean'), _cabi.stream_ptr(dev)))
+            4 * scratch.numel(), rows, v, stride, dt, k, temperature, int(reduction == 'mean'), _cabi.stream_ptr(dev))
+    if code == _cabi.UNSUPPORTED:
+        return None
+    _cabi.check(code)
     return rec, grad
 
 
