@@ -504,10 +504,10 @@ __global__ void __launch_bounds__(ring_block<G>, backward_blocks<G>) norm_backwa
         load_columns<T, V, G>(x, own.n, t, h);
         load_columns<T, V, G>(dy, own.n, t, g);
         {
-            const pk_t negm = psplat(-st.x), rr = psplat(st.y);
+            const pk_t nmr = psplat(-st.x * st.y), rr = psplat(st.y);
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
-                h[i] = pmul(padd(h[i], negm), rr);
+                h[i] = pfma(h[i], rr, nmr);
                 dw[i] = pfma(g[i], h[i], dw[i]);
                 db[i] = padd(db[i], g[i]);
                 g[i] = pmul(g[i], w[i]);
@@ -520,23 +520,35 @@ __global__ void __launch_bounds__(ring_block<G>, backward_blocks<G>) norm_backwa
         if (G > 32) {
             const float2 *all = sums[group][turn];
             exchange<G>(sums[group][turn], warp, rank, p.blocks, make_float2(sg, sgh), group);
-            const int n = WARPS * (G == kTeamThreads ? p.blocks : 1);
-            sg = sgh = 0.f;
-            for (int i = lane; i < n; i += 32) {
-                sg += all[i].x;
-                sgh += all[i].y;
+            if (G == kTeamThreads && p.blocks > 1) {
+                sg = sgh = 0.f;
+                for (int i = lane; i < WARPS * p.blocks; i += 32) {
+                    sg += all[i].x;
+                    sgh += all[i].y;
+                }
+                sg = warp_sum(sg);
+                sgh = warp_sum(sgh);
+            } else {                                        // (each lane starts with one of the WARPS numbers)
+                const float2 one = all[lane & (WARPS - 1)];
+                sg = one.x;
+                sgh = one.y;
+#pragma unroll
+                for (int o = WARPS / 2; o > 0; o >>= 1) {
+                    sg += __shfl_xor_sync(0xffffffffu, sg, o);
+                    sgh += __shfl_xor_sync(0xffffffffu, sgh, o);
+                }
             }
-            sg = warp_sum(sg);
-            sgh = warp_sum(sgh);
         } else {
             __syncwarp();
         }
         if (lost[group]) dead = true;
         const int64_t ahead = r + int64_t(p.stages) * step;
         if (!dead && ahead < p.rows) ring.fill(stage, xs + ahead * p.x_stride, ys + ahead * p.dy_stride, own.n);
-        const pk_t rr = psplat(dead ? nan_f() : st.y), nsg = psplat(-sg * inv_d), nsgh = psplat(-sgh * inv_d);
+        // dx = r g - r mean(g) - h r mean(g h)
+        const float r0 = dead ? nan_f() : st.y;
+        const pk_t rr = psplat(r0), c0 = psplat(-sg * inv_d * r0), c1 = psplat(-sgh * inv_d * r0);
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i) g[i] = pmul(pfma(h[i], nsgh, padd(g[i], nsg)), rr);
+        for (int i = 0; i < kPairs; ++i) g[i] = pfma(g[i], rr, pfma(h[i], c1, c0));
         store_columns<T, V, G>(static_cast<T *>(p.dx) + r * int64_t(p.D) + own.first, own.n, t, g);
         turn ^= 1;
         if (++stage == p.stages) {
@@ -622,6 +634,7 @@ template <typename T> __global__ void __launch_bounds__(256) norm_columns_any_ke
 template <typename P>
 __global__ void __launch_bounds__(512) norm_columns_kernel(const float *partial, int blocks, int D, P *dw, P *db) {
     __shared__ float sh[16][33];
+    pdl_wait();
     const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
     const int64_t width = 2 * int64_t(D);
     const int64_t j = int64_t(blockIdx.x) * 32 + lane;
@@ -741,9 +754,9 @@ template <typename T, typename P> struct NormLaunch {
             if (rc) return rc;
         }
         if (!p.partial) return B200_OK;
-        norm_columns_kernel<P><<<unsigned((2 * int64_t(p.D) + 31) / 32), 512, 0, s>>>(
-            p.partial, p.rows > 0 ? ring_teams(p.rows, plan) : 0, p.D, static_cast<P *>(dw), static_cast<P *>(db));
-        return launch_status("layer norm column kernel launch");
+        return launch_cluster(norm_columns_kernel<P>, (2 * int64_t(p.D) + 31) / 32, 512, 0, 1, true, s,
+                              "layer norm column kernel launch", static_cast<const float *>(p.partial),
+                              p.rows > 0 ? ring_teams(p.rows, plan) : 0, p.D, static_cast<P *>(dw), static_cast<P *>(db));
     }
 };
 
