@@ -263,16 +263,25 @@ __global__ void __launch_bounds__(THREADS) distill_step_kernel(const StepParams 
     const float A = nothing ? 0.f : scale / st.s;
     auto one = [&](float v) { return ex2f((v - m) * p.c) * A; };
     const pk_t negm = psplat(-m), cc = psplat(p.c), aa = psplat(A);
-#pragma unroll 4
-    for (int i = part.body + t * N; i < part.body_end; i += THREADS * N) {
-        const uint4 v = load(i);
+    const int vectors = (part.body_end - part.body) / N;
+    const uint4 *src = (HELD ? held : reinterpret_cast<const uint4 *>(row + part.body)) + t;
+    T *dst = g + part.body + t * N;
+    auto gradient = [&](const uint4 &v, T *to) {
         float2 d[N / 2];
 #pragma unroll
-        for (int h = 0; h < N / 2; ++h) {
+        for (int h = 0; h < N / 2; ++h)
             d[h] = upk2(pmul(pex2(pmul(padd(pk2(TokenVec<T>::pair(v, h)), negm), cc)), aa));
-        }
-        st_stream16(g + i, TokenVec<T>::pack(d));
+        st_stream16(to, TokenVec<T>::pack(d));
+    };
+    int i = t;
+    for (; i + 3 * THREADS < vectors; i += 4 * THREADS, src += 4 * THREADS, dst += 4 * THREADS * N) {
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = src[k * THREADS];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) gradient(v[k], dst + k * THREADS * N);
     }
+    for (; i < vectors; i += THREADS, src += THREADS, dst += THREADS * N) gradient(*src, dst);
     if (t < ragged_count(part)) {
         const int j = ragged_index(part, t);
         g[j] = from_f32<T>(one(to_f32(row[j])));
