@@ -33,6 +33,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+// Whether a maximum rises (or is NaN).  Not a plain comparison: the library is built with denormals flushed, and the
+// maxima keep them apart.
+__device__ __forceinline__ bool rises(float to, float m) {
+    unsigned r;
+    asm("{\n\t.reg .pred p;\n\tsetp.gtu.f32 p, %1, %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "f"(to), "f"(m));
+    return r != 0u;
+}
 // The reference that a maximum stands for: 0 where there is nothing but -inf, so that differences exist.
 __device__ __forceinline__ float reference_of(float m) { return m == -INFINITY ? 0.f : m; }
 
@@ -199,7 +206,7 @@ template <bool ENTROPY> struct RowStat {
     }
     __device__ __forceinline__ void add(float x, float c) {          // one element
         const float to = max_nan(m, x);
-        if (!(to <= m)) raise(to, c);
+        if (rises(to, m)) raise(to, c);
         const float z = max_nan((x - reference_of(m)) * c, kTokenFloor), e = ex2f(z);
         s += e;
         if (ENTROPY) u = fmaf(e, z, u);
@@ -207,7 +214,7 @@ template <bool ENTROPY> struct RowStat {
     // Some vectors; returns the largest logit among them.
     template <typename T, int COUNT> __device__ __forceinline__ float add(const uint4 (&v)[COUNT], float c) {
         const float own = TokenVec<T>::largest(v), to = max_nan(m, own);
-        if (!(to <= m)) raise(to, c);
+        if (rises(to, m)) raise(to, c);
         const pk_t negm = psplat(-reference_of(m)), cc = psplat(c);
         pk_t s2 = psplat(0.f), u2 = psplat(0.f);
 #pragma unroll

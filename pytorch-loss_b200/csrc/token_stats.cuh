@@ -154,6 +154,7 @@ template <int G, bool TOP> __device__ __forceinline__ int narrow(int n, int t, i
     unsigned long long own[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) own[i] = t + i * G < n ? sh.cand[t + i * G] : 0ull;
+    group_sync<G>();                                        // (everybody has read the candidates and their number)
     if (t == 0) sh.count = 0;
     group_sync<G>();
     const unsigned bound = sh.bound;

@@ -88,19 +88,18 @@ __global__ void __launch_bounds__(32 * kListWarps) distill_lists_kernel(const in
         sum = warp_sum(sum);
         __syncwarp();
         // the same token twice?  Rare: only looked for here
-        int twins = 0;
+        int meets[kMaxList / 32] = {};
         for (int j = 0; j < K; j += 4) {
             const int4 four = *reinterpret_cast<const int4 *>(&ids[warp][j]);
 #pragma unroll
             for (int e = 0; e < kMaxList / 32; ++e) {
                 if (32 * e >= K) break;
-                const int id = own[e];
-                twins += (four.x == id) + (four.y == id) + (four.z == id) + (four.w == id);
+                meets[e] += (four.x == own[e]) + (four.y == own[e]) + (four.z == own[e]) + (four.w == own[e]);
             }
         }
-        // (every entry meets itself; tokens that do not exist meet each other, which only costs the longer way)
+        int twins = 0;                                      // (every entry meets itself)
 #pragma unroll
-        for (int e = 0; e < kMaxList / 32; ++e) twins -= lane + 32 * e < K ? 1 : 0;
+        for (int e = 0; e < kMaxList / 32; ++e) twins += own[e] >= 0 && meets[e] > 1 ? 1 : 0;
         const bool merge = __any_sync(0xffffffffu, twins > 0);
         for (int e = 0; e * 32 < K; ++e) {
             const int i = lane + 32 * e;

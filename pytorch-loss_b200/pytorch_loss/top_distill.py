@@ -145,4 +145,7 @@ class TopTokenDistillLoss(nn.Module):
         self.reduction = reduction
 
     def forward(self, logits, top_tokens, top_logprobs):
-        return TopTokenDistillFunc.apply(logits, top_tokens, top_logprobs, float(self.temperature), self.reduction)
+        if logits.requires_grad and torch.is_grad_enabled():
+            return TopTokenDistillFunc.apply(logits, top_tokens, top_logprobs, float(self.temperature), self.reduction)
+        losses, rec, _, _, _ = _two_pass(logits, top_tokens, top_logprobs, float(self.temperature), self.reduction)
+        return losses if rec is None else rec[4] if self.reduction == 'mean' else rec[5]

@@ -228,6 +228,22 @@ def test_large_logits_where_few_threads_see_them(dtype):
         check(x.repeat(300, 1), tokens.repeat(300), k=k)            # (one block to a row)
 
 
+def test_logits_below_the_normal_range():
+    """Denormal logits keep their order among the alternatives (their log probabilities cannot tell them apart)."""
+    import pytorch_loss as P
+    for v in (200, 3000, 20000):
+        x = torch.zeros(4, v)
+        x[:, ::3] = torch.rand(4, len(range(0, v, 3))) * 1e-38
+        x[:, 5] = -1e-40
+        x[1] -= 1e-39
+        x[2] = x[2].sort().values
+        for dtype in (torch.float32, torch.bfloat16):
+            y = x.to(dtype).cuda()
+            for k in (5, 30, 100):
+                got = P.token_logprobs(y, torch.zeros(4, dtype=torch.int64, device="cuda"), top_k=k)
+                assert torch.equal(got.top_tokens.cpu(), O.alternatives(y.cpu(), k))
+
+
 @pytest.mark.parametrize("t", [1e-4, 0.05, 20.0, 1e4])
 def test_temperatures(t):
     x, tokens, dl, dh = inputs(6, 3000, torch.float32)
