@@ -51,8 +51,12 @@ __device__ __forceinline__ float log_prob(float x, float m, float inv_t, float l
 // ---- 16-byte vectors of logits as pairs of floats
 
 template <typename T> struct TokenVec;
+__device__ __forceinline__ unsigned word_of(const uint4 &v, int i) {
+    return i & 2 ? (i & 1 ? v.w : v.z) : (i & 1 ? v.y : v.x);
+}
 template <> struct TokenVec<float> {
     static constexpr int N = 4;
+    static __device__ __forceinline__ float element(const uint4 &v, int i) { return __uint_as_float(word_of(v, i)); }
     static constexpr unsigned kMasked = 0xff800000u;              // -inf
     static __device__ __forceinline__ float2 pair(const uint4 &v, int i) {
         return i == 0 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y))
@@ -74,6 +78,10 @@ template <> struct TokenVec<float> {
 };
 template <> struct TokenVec<__half> {
     static constexpr int N = 8;
+    static __device__ __forceinline__ float element(const uint4 &v, int i) {
+        const unsigned w = word_of(v, i >> 1);
+        return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? w >> 16 : w)));
+    }
     static constexpr unsigned kMasked = 0xfc00fc00u;
     static __device__ __forceinline__ __half2 word(unsigned w) { return *reinterpret_cast<__half2 *>(&w); }
     static __device__ __forceinline__ float2 pair(const uint4 &v, int i) {
@@ -105,6 +113,10 @@ template <> struct TokenVec<__half> {
 };
 template <> struct TokenVec<__nv_bfloat16> {
     static constexpr int N = 8;
+    static __device__ __forceinline__ float element(const uint4 &v, int i) {
+        const unsigned w = word_of(v, i >> 1);
+        return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    }
     static constexpr unsigned kMasked = 0xff80ff80u;
     static __device__ __forceinline__ __nv_bfloat162 word(unsigned w) { return *reinterpret_cast<__nv_bfloat162 *>(&w); }
     static __device__ __forceinline__ float2 pair(const uint4 &v, int i) {

@@ -139,25 +139,30 @@ __device__ __forceinline__ int larger_keys(const unsigned long long *keys, int n
 
 // Of n candidates (0: none) those that reach the K-th largest of their upper 16 bits; returns how many these are.
 template <int G, bool TOP> __device__ __forceinline__ int narrow(int n, int t, int K, TokenShared<G, TOP> &sh) {
-    constexpr int PER = kCandidates<G> / G;
-    if (t < 32) {
-        unsigned bound = 0u;
-#pragma unroll 1
-        for (int bit = 15; bit >= 0; --bit) {
-            const unsigned trial = bound | (1u << bit);
-            unsigned of = 0u;
-            for (int i = t; i < n; i += 32) of += unsigned(sh.cand[i] >> 48) >= trial ? 1u : 0u;
-            if (__reduce_add_sync(0xffffffffu, of) >= unsigned(K)) bound = trial;
-        }
-        if (t == 0) sh.bound = bound;
-    }
+    constexpr int PER = kCandidates<G> / G, WARPS = G / 32;
     unsigned long long own[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) own[i] = t + i * G < n ? sh.cand[t + i * G] : 0ull;
+    unsigned bound = 0u;
+#pragma unroll 1
+    for (int bit = 15; bit >= 0; --bit) {
+        const unsigned trial = bound | (1u << bit);
+        unsigned of = 0u;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) of += unsigned(own[i] >> 48) >= trial ? 1u : 0u;
+        of = __reduce_add_sync(0xffffffffu, of);
+        if (G > 32) {
+            if ((t & 31) == 0) sh.hist[bit * WARPS + (t >> 5)] = of;
+            __syncthreads();
+            of = 0u;
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i) of += sh.hist[bit * WARPS + i];
+        }
+        if (of >= unsigned(K)) bound = trial;
+    }
     group_sync<G>();                                        // (everybody has read the candidates and their number)
     if (t == 0) sh.count = 0;
     group_sync<G>();
-    const unsigned bound = sh.bound;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
         if (own[i] && unsigned(own[i] >> 48) >= bound) sh.cand[atomicAdd(&sh.count, 1)] = own[i];
@@ -235,12 +240,17 @@ __device__ __forceinline__ void largest(const T *row, const RowPart &part, int t
             const int64_t at = part.body + (owner + int64_t(first + k) * G) * N;
             if (at >= part.body_end) break;
             const uint4 v = load(int(at));
-            if (TokenVec<T>::largest(v) < least) continue;
+            // (which elements first: a warp then goes once or twice through what it costs to keep one, not N times)
+            unsigned wanted = 0u;
 #pragma unroll
             for (int h = 0; h < N / 2; ++h) {
                 const float2 x = TokenVec<T>::pair(v, h);
-                keep(x.x, int(at) + 2 * h);
-                keep(x.y, int(at) + 2 * h + 1);
+                wanted |= (x.x < least ? 0u : 1u << (2 * h)) | (x.y < least ? 0u : 2u << (2 * h));
+            }
+            while (wanted) {
+                const int e = __ffs(wanted) - 1;
+                wanted &= wanted - 1u;
+                keep(TokenVec<T>::element(v, e), int(at) + e);
             }
         }
     }
@@ -273,7 +283,7 @@ __device__ __forceinline__ void largest(const T *row, const RowPart &part, int t
 // Bound: HBM, the logits once; instruction issue and the 16 exponentials a clock of an SM are next (16-bit logits
 // take 11.6 of them at HBM speed).
 template <typename T, int G, int MODE, bool TOP>
-__global__ void __launch_bounds__(G == 32 ? 256 : G) token_stats_kernel(const TokenParams p) {
+__global__ void __launch_bounds__(G == 32 ? 256 : G, G == 32 ? 5 : 1536 / G) token_stats_kernel(const TokenParams p) {
     constexpr bool ENTROPY = MODE == kTokens;
     constexpr int WARPS = G / 32, GROUPS = G == 32 ? 8 : 1;
     __shared__ TokenShared<G, TOP> shared[GROUPS];
