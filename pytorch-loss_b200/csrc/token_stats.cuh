@@ -475,7 +475,7 @@ template <typename T, int G> struct ListShare {
 
 // Which entries of a row's list each thread meets among the elements it writes: the thread that owns an element is
 // handed its entry, so that the element leaves complete (a second, 2-byte store to lines on their way to memory cost
-// the gradient kernel 20 %: [16384, 32768] bfloat16 with lists of 20 391 against @@ us).
+// the gradient kernel 20 %: [16384, 32768] bfloat16 with lists of 20 391 against 317 us).
 template <int G> struct ListChain {
     int head[G];
     int next[kMaxList], at[kMaxList];
@@ -666,11 +666,11 @@ inline int row_part_shift(int64_t rows, int64_t V, int dtype) {
 // How many threads share a row.  What a row costs besides its elements (joins, barriers, finding the alternatives) is
 // paid per thread, so few threads are better -- as long as there are rows enough to fill the SMs several times over,
 // and a list of alternatives is short against the number of threads.  Measured, us at 32 / 128 / 256 threads:
-//   [32768, 4000] bfloat16 (8 KB)     log probabilities 58 / 82 / 120    with 20 alternatives 121 / 176 / 269
-//   [16384, 8192] float32 (32 KB)     84 / 80 / 87                       161 / 120 / 155
-//   [16384, 32768] bfloat16 (64 KB)   173 / 168 / 174                    792 / 224 / 259
-//   [2047, 100003] float16 (200 KB)   -- / 80 / 72                       -- / 101 / 89     (one wave of 128 threads)
-//   128 alternatives of [16384, 32768]: -- / 1409 / 433
+//   [32768, 4000] bfloat16 (8 KB)     log probabilities 50 / 67 / 107    with 20 alternatives 106 / 146 / 244
+//   [16384, 8192] float32 (32 KB)     79 / 80 / 85                       169 / 119 / 149
+//   [16384, 32768] bfloat16 (64 KB)   170 / 167 / 171                    349 / 220 / 252
+//   [2047, 100003] float16 (200 KB)   105 / 80 / 71                      333 / 104 / 88    (one wave of 128 threads)
+//   128 alternatives of [16384, 32768], before the candidates were narrowed: -- / 1409 / 433
 template <typename T, int MODE, bool TOP> int launch_stats(const TokenParams &prm, int dtype, cudaStream_t stream) {
     TokenParams p = prm;
     const char *what = "token statistics kernel launch";

@@ -314,16 +314,17 @@ __global__ void __launch_bounds__(THREADS) distill_step_kernel(const StepParams 
 }
 
 // How a step treats a row.  Measured (us, lists of 20; two passes: statistics, then gradient):
-//   [16384, 4096] bfloat16 (8 KB)     held by 128 threads 79, 256 110           two passes 103
-//   [16384, 16384] bfloat16 (32 KB)   held by 128 193, 256 190, 512 262         270
-//   [16384, 32768] bfloat16 (64 KB)   held by 128 424, 256 374, 512 387         505    from L2, 512 threads: 406
-//   [8192, 24000] float32 (96 KB)     held by 256 322                           360    from L2: 272
-//   [8192, 65536] bfloat16 (128 KB)   held by two blocks 436                    493    from L2: 412, two blocks 479
-//   [3000, 50001] float32 (200 KB)    275                                       281    from L2: 299, two blocks 255
-//   [4096, 131072] bfloat16 (256 KB)  513                                       483    from L2: 519, two blocks 437
-//   [2048, 131072] float32 (512 KB)   503                                       482    from L2: 532, two blocks 529
-// From L2 works while the rows under way fit there (three blocks of 512 threads an SM: 57 MB at 128 KB); blocks of a
-// cluster wait for each other's place on the chip.
+//   [16384, 4096] bfloat16 (8 KB)     held by 128 threads 73, by 256 104     two passes 99     from L2 169
+//   [16384, 16384] bfloat16 (32 KB)   185, 185                               261               247
+//   [16384, 32768] bfloat16 (64 KB)   404, 367                               501               391
+//   [8192, 24000] float32 (96 KB)     (two blocks on an SM) 322              357               257
+//   [8192, 65536] bfloat16 (128 KB)                                          487               408, by two blocks 462
+//   [3000, 50001] float32 (200 KB)                                           281               274, by two blocks 240
+//   [4096, 131072] bfloat16 (256 KB)                                         479               488, by two blocks 408
+//   [2048, 81920] float32 (320 KB)                                           312               311, by two blocks 287
+//   [2048, 131072] float32 (512 KB)                                          478               532, by two blocks 529
+// From L2 works while the rows under way fit there (three blocks of 512 threads an SM: 57 MB at 128 KB, where 12 % of
+// the rows are read from memory twice).  What the step loses there it loses to its phases: a block reads, joins, writes.
 enum StepWay { kNoStep, kHeld128, kHeld256, kFromL2, kFromL2Pair };
 inline StepWay step_way(int64_t V, int dtype) {
     const int64_t bytes = V * int64_t(dtype_size(dtype));
