@@ -9,11 +9,9 @@
 // block order, so results repeat bit for bit.
 //
 // Bound: HBM (2 s D per row forward, 3 s D backward, s the element's bytes).  Measured, us and share of the 6.55 TB/s of
-// a copy:  [16384, 4096] bfloat16, float32 weights   48 (0.86) + 78 (0.79)     [16384, 8192] float16   86 (0.96) + 148 (0.83)
+// a copy:  [16384, 4096] bfloat16, float32 weights   50 (0.81) + 78 (0.79)     [16384, 8192] float16   90 (0.91) + 147 (0.84)
 //          [32768, 2048] float32                     82 (0.99) + 141 (0.87)    [16384, 4001] float32   96 (0.83) + 146 (0.82)
 // Rows of odd widths in 16 bits go element by element and reach 0.36.
-#include <type_traits>
-
 #include "token_rows.cuh"
 
 namespace b200 {
@@ -101,7 +99,7 @@ template <int W> __device__ __forceinline__ void store_words(void *p, const RowW
         asm volatile("st.global.cs.v2.u32 [%0], {%1,%2};" ::"l"(p), "r"(r.w[0]), "r"(r.w[1]) : "memory");
 }
 // The words themselves are what lives on from here: without this the compiler keeps the floats made of them, twice as
-// many registers for 16-bit types (72 against 48 a thread).
+// many registers for 16-bit types (72 against 52 a thread).
 template <int N, int W> __device__ __forceinline__ void keep_words(RowWords<W> (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -117,20 +115,19 @@ template <typename T, typename P> constexpr int row_vectors_held = kRowElements<
 // Rows of whole vectors: a row stays in the registers of its G threads (a warp, or a block) as the words it was read as,
 // 64 bytes a thread, so that many of them are on their way at once.
 template <typename T, typename P, int G>
-__global__ void __launch_bounds__(G == 32 ? 256 : G, G == 512 ? 3 : 1) norm_forward_kernel(const NormParams p) {
+__global__ void __launch_bounds__(G == 32 ? 256 : G) norm_forward_kernel(const NormParams p) {
     constexpr int V = row_vector<T, P>, N = row_vectors_held<T, P>, W = V * int(sizeof(T)) / 4;
     __shared__ float sh[2][32];
     const int t = G == 32 ? threadIdx.x & 31 : threadIdx.x;
     const int64_t r = G == 32 ? int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5) : int64_t(blockIdx.x);
     if (r >= p.rows) return;
-    // (a thread's own pointers: vector i of a row lies a constant i * G * V elements behind them)
-    const T *x = static_cast<const T *>(p.x) + r * p.x_stride + t * V;
-    T *y = static_cast<T *>(p.y) + r * int64_t(p.D) + t * V;
-    const int mine = p.D - t * V;                           // vector i exists if i * G * V < mine
+    const T *x = static_cast<const T *>(p.x) + r * p.x_stride;
+    T *y = static_cast<T *>(p.y) + r * int64_t(p.D);
     RowWords<W> v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        if (i * G * V < mine) v[i] = load_words<W>(x + i * G * V);
+        const int j = (i * G + t) * V;
+        if (j < p.D) v[i] = load_words<W>(x + j);
         else
 #pragma unroll
             for (int k = 0; k < W; ++k) v[i].w[k] = 0u;
@@ -149,7 +146,7 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 512 ? 3 : 1) norm_forw
     sum = psplat(0.f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        if (i * G * V < mine) {
+        if ((i * G + t) * V < p.D) {
 #pragma unroll
             for (int h = 0; h < V / 2; ++h) {
                 const pk_t d = padd(pair(i, h), negm);
@@ -161,35 +158,27 @@ __global__ void __launch_bounds__(G == 32 ? 256 : G, G == 512 ? 3 : 1) norm_forw
     const float rstd = rsqrtf(row_sum<G>(s.x + s.y, sh[1]) * inv_d + p.eps);
     keep_words(v);
     if (t == 0 && p.stats) p.stats[r] = make_float2(mean, rstd);
-    static_assert(V * sizeof(P) == 16, "a vector of weights is one access");
-    const uint4 *w = reinterpret_cast<const uint4 *>(p.w), *b = reinterpret_cast<const uint4 *>(p.b);
+    const P *w = static_cast<const P *>(p.w), *b = static_cast<const P *>(p.b);
     const pk_t rr = psplat(rstd);
-    // (one of four forms for the whole row, not a choice per vector)
-    auto write = [&](auto weighted, auto biased) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (i * G * V < mine) {
-                uint4 a, c;
-                if (weighted) a = __ldg(w + t + i * G);
-                if (biased) c = __ldg(b + t + i * G);
-                RowWords<W> out;
+    for (int i = 0; i < N; ++i) {
+        const int j = (i * G + t) * V;
+        if (j < p.D) {
+            static_assert(V * sizeof(P) == 16, "a vector of weights is one access");
+            uint4 a, c;
+            if (w) a = __ldg(reinterpret_cast<const uint4 *>(w + j));
+            if (b) c = __ldg(reinterpret_cast<const uint4 *>(b + j));
+            RowWords<W> out;
 #pragma unroll
-                for (int h = 0; h < V / 2; ++h) {
-                    const pk_t u = pmul(padd(pair(i, h), negm), rr);
-                    const pk_t aw = weighted ? pair_of(reinterpret_cast<const P *>(&a) + 2 * h) : psplat(1.f);
-                    const pk_t cb = biased ? pair_of(reinterpret_cast<const P *>(&c) + 2 * h) : psplat(0.f);
-                    st_pk(reinterpret_cast<T *>(out.w) + 2 * h, pfma(u, aw, cb));
-                }
-                store_words(y + i * G * V, out);
+            for (int h = 0; h < V / 2; ++h) {
+                const pk_t u = pmul(padd(pair(i, h), negm), rr);
+                const pk_t aw = w ? pair_of(reinterpret_cast<const P *>(&a) + 2 * h) : psplat(1.f);
+                const pk_t cb = b ? pair_of(reinterpret_cast<const P *>(&c) + 2 * h) : psplat(0.f);
+                st_pk(reinterpret_cast<T *>(out.w) + 2 * h, pfma(u, aw, cb));
             }
+            store_words(y + j, out);
         }
-    };
-    constexpr std::true_type yes{};
-    constexpr std::false_type no{};
-    if (w && b) write(yes, yes);
-    else if (w) write(yes, no);
-    else if (b) write(no, yes);
-    else write(no, no);
+    }
 }
 
 // Any row length: three sweeps over the row, the later ones from L2.
