@@ -12,6 +12,8 @@
 // a copy:  [16384, 4096] bfloat16, float32 weights   50 (0.81) + 78 (0.79)     [16384, 8192] float16   90 (0.91) + 147 (0.84)
 //          [32768, 2048] float32                     82 (0.99) + 141 (0.87)    [16384, 4001] float32   96 (0.83) + 146 (0.82)
 // Rows of odd widths in 16 bits go element by element and reach 0.36.
+#include <algorithm>
+
 #include "token_rows.cuh"
 
 namespace b200 {
@@ -684,7 +686,7 @@ inline RingPlan ring_plan(int D, size_t s, bool backward) {
 }
 // Teams of blocks that share a row.
 inline int ring_teams(int64_t rows, const RingPlan &plan) {
-    const int64_t most = plan.threads == 0 ? 64 : int64_t(sm_count()) * plan.per_sm / plan.blocks;
+    const int64_t most = plan.threads == 0 ? 64 : std::max<int64_t>(int64_t(sm_count()) * plan.per_sm / plan.blocks, 1);
     const int64_t want = (rows + plan.groups() - 1) / plan.groups();
     return int(want < 1 ? 1 : want > most ? most : want);
 }
@@ -695,7 +697,7 @@ template <typename K> int launch_ring(K kernel, NormParams p, const RingPlan &pl
     if (const int rc = set_smem(kernel, smem)) return rc;
     return launch_cluster(kernel, int64_t(ring_teams(p.rows, plan)) * plan.blocks, block, smem, plan.blocks, false, s, what, p);
 }
-inline bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool on16(const void *p) { return lies_on(p, 16); }
 
 template <typename T, typename P> struct NormLaunch {
     template <int G> static int forward_rows(const NormParams &p, cudaStream_t s) {
@@ -798,7 +800,9 @@ extern "C" int b200_layer_norm(const void *x, const void *weight, const void *bi
                                int64_t D, int64_t stride, int dtype, int param_dtype, float eps, void *stream) {
     const char *who = "b200_layer_norm";
     if (const int rc = check_norm(who, rows, D, dtype, param_dtype)) return rc;
-    if (!(eps >= 0.f) || stride < 0 || (rows > 0 && (!x || !y)) || (reinterpret_cast<uintptr_t>(stats) & 7)) {
+    const size_t e = dtype_size(dtype), pe = dtype_size(param_dtype);
+    if (!(eps >= 0.f) || stride < 0 || (rows > 0 && (!x || !y)) || !lies_on(stats, 8) || !lies_on(x, e) || !lies_on(y, e) ||
+        !lies_on(weight, pe) || !lies_on(bias, pe)) {
         set_error("%s: null or misaligned pointer, or eps < 0", who);
         return B200_ERR_ARG;
     }
@@ -828,7 +832,9 @@ extern "C" int b200_layer_norm_backward(const void *x, const void *weight, const
                                         void *stream) {
     const char *who = "b200_layer_norm_backward";
     if (const int rc = check_norm(who, rows, D, dtype, param_dtype)) return rc;
-    if (stride < 0 || dy_stride < 0 || (rows > 0 && (!x || !dy || !dx || !stats)) || (reinterpret_cast<uintptr_t>(stats) & 7)) {
+    const size_t e = dtype_size(dtype), pe = dtype_size(param_dtype);
+    if (stride < 0 || dy_stride < 0 || (rows > 0 && (!x || !dy || !dx || !stats)) || !lies_on(stats, 8) || !lies_on(x, e) ||
+        !lies_on(dy, e) || !lies_on(dx, e) || !lies_on(weight, pe) || !lies_on(dweight, pe) || !lies_on(dbias, pe)) {
         set_error("%s: null or misaligned pointer", who);
         return B200_ERR_ARG;
     }

@@ -14,8 +14,9 @@ extern "C" int b200_token_logprobs(const void *logits, const int64_t *tokens, fl
         return B200_ERR_ARG;
     }
     if (rows > 0 && (!tokens || !logprobs || !entropy || (top_k > 0 && (!top_logprobs || !top_tokens)) ||
-                     (reinterpret_cast<uintptr_t>(stats) & 15))) {
-        set_error("%s: null pointer, or statistics not on 16 bytes", who);
+                     !lies_on(stats, 16) || !lies_on(tokens, 8) || !lies_on(top_tokens, 8) || !lies_on(logprobs, 4) ||
+                     !lies_on(entropy, 4) || !lies_on(top_logprobs, 4))) {
+        set_error("%s: null or misaligned pointer (statistics: 16 bytes)", who);
         return B200_ERR_ARG;
     }
     TokenParams p{};
@@ -47,8 +48,8 @@ extern "C" int b200_token_logprobs_backward(const void *logits, const int64_t *t
                                             int64_t ignore_index, void *stream) {
     const char *who = "b200_token_logprobs_backward";
     if (const int rc = check_rows(who, logits, rows, V, stride, dtype, temperature)) return rc;
-    if (rows > 0 && (!tokens || !stats || !grad_logits || (reinterpret_cast<uintptr_t>(stats) & 15) ||
-                     (reinterpret_cast<uintptr_t>(grad_logits) & (dtype_size(dtype) - 1)))) {
+    if (rows > 0 && (!tokens || !stats || !grad_logits || !lies_on(stats, 16) || !lies_on(tokens, 8) ||
+                     !lies_on(d_logprobs, 4) || !lies_on(d_entropy, 4) || !lies_on(grad_logits, dtype_size(dtype)))) {
         set_error("%s: null or misaligned pointer", who);
         return B200_ERR_ARG;
     }

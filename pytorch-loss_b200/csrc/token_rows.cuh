@@ -336,6 +336,9 @@ inline int launch_cluster(void (*kernel)(KArgs...), int64_t grid, int block, siz
     return rc;
 }
 
+// Whether a pointer (null included) lies on a multiple of `bytes`, a power of two.
+inline bool lies_on(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
 // 16-byte vectors of a row, at most.
 inline int64_t row_vectors(int64_t V, int dtype) { return V * int64_t(dtype_size(dtype)) / 16; }
 

@@ -728,7 +728,7 @@ inline int check_rows(const char *who, const void *x, int64_t rows, int64_t V, i
         set_error("%s: the temperature must lie between 1e-4 and 1e4", who);
         return B200_ERR_ARG;
     }
-    if (rows > 0 && (!x || (reinterpret_cast<uintptr_t>(x) & (dtype_size(dtype) - 1)))) {
+    if (rows > 0 && (!x || !lies_on(x, dtype_size(dtype)))) {
         set_error("%s: the logits are null or not aligned to their type", who);
         return B200_ERR_ARG;
     }

@@ -371,11 +371,11 @@ int check_distill(const char *who, const void *x, const int64_t *tokens, const v
         set_error("%s: lists of 1 to %d tokens", who, kMaxList);
         return B200_ERR_ARG;
     }
-    if (rows > 0 && !tokens) {
-        set_error("%s: null pointer", who);
+    if (rows > 0 && (!tokens || !lies_on(tokens, 8))) {
+        set_error("%s: null or misaligned pointer", who);
         return B200_ERR_ARG;
     }
-    if (!scratch || (reinterpret_cast<uintptr_t>(scratch) & 15) || scratch_bytes < b200_top_distill_scratch_bytes(rows, K)) {
+    if (!scratch || !lies_on(scratch, 16) || scratch_bytes < b200_top_distill_scratch_bytes(rows, K)) {
         set_error("%s: scratch of %zu bytes on a 16-byte address required", who, b200_top_distill_scratch_bytes(rows, K));
         return B200_ERR_WORKSPACE;
     }
@@ -398,8 +398,9 @@ extern "C" int b200_top_distill_forward(const void *logits, const int64_t *top_t
     const char *who = "b200_top_distill_forward";
     if (const int rc = check_distill(who, logits, top_tokens, scratch, scratch_bytes, rows, V, stride, dtype, K, temperature))
         return rc;
-    if ((rows > 0 && !top_logprobs) || (!losses && !out)) {
-        set_error("%s: null pointer", who);
+    if ((rows > 0 && !top_logprobs) || (!losses && !out) || !lies_on(top_logprobs, 4) || !lies_on(losses, 4) ||
+        !lies_on(out, 8)) {
+        set_error("%s: null or misaligned pointer", who);
         return B200_ERR_ARG;
     }
     const DistillScratch d = carve(scratch, rows);
@@ -432,8 +433,8 @@ extern "C" int b200_top_distill_backward(const void *logits, const int64_t *top_
     const char *who = "b200_top_distill_backward";
     if (const int rc = check_distill(who, logits, top_tokens, scratch, scratch_bytes, rows, V, stride, dtype, K, temperature))
         return rc;
-    if ((rows > 0 && (!d_loss || !grad_logits)) || (reinterpret_cast<uintptr_t>(count) & 7) ||
-        (reinterpret_cast<uintptr_t>(grad_logits) & (dtype_size(dtype) - 1))) {
+    if ((rows > 0 && (!d_loss || !grad_logits)) || !lies_on(count, 8) || !lies_on(d_loss, 4) ||
+        !lies_on(grad_logits, dtype_size(dtype))) {
         set_error("%s: null or misaligned pointer", who);
         return B200_ERR_ARG;
     }
@@ -476,6 +477,10 @@ extern "C" int b200_top_distill_step(const void *logits, const int64_t *top_toke
     const char *who = "b200_top_distill_step";
     if (const int rc = check_distill(who, logits, top_tokens, scratch, scratch_bytes, rows, V, stride, dtype, K, temperature))
         return rc;
+    if (!lies_on(top_logprobs, 4) || !lies_on(out, 8)) {
+        set_error("%s: misaligned pointer", who);
+        return B200_ERR_ARG;
+    }
     if (!top_logprobs || !grad_logits || !out || !b200_top_distill_step_path(logits, grad_logits, rows, V, stride, dtype)) {
         set_error("%s: these logits have no one-pass step", who);
         return B200_ERR_UNSUPPORTED;

@@ -94,6 +94,29 @@ def test_layer_norm_refuses(lib):
         assert bwd(**change) == code, change
 
 
+def test_pointers_off_their_type_are_refused(lib):
+    four, two = ctypes.c_void_p(0x7f0000001004), ctypes.c_void_p(0x7f0000001002)
+    for change in ({"tokens": four}, {"ids": four}, {"lp": two}, {"h": two}, {"top": two}, {"x": two}):
+        assert _logprobs(lib, **change) == 1, change
+    back = lambda tok=A, dl=A, dh=A, g=A: lib.b200_token_logprobs_backward(A, tok, A, dl, dh, g, 4, 100, 100, F32, 1.0, -100, None)
+    for change in ({"tok": four}, {"dl": two}, {"dh": two}, {"g": two}):
+        assert back(**change) == 1, change
+    need = lib.b200_top_distill_scratch_bytes(4, 8)
+    fwd = lambda tok=A, q=A, losses=A, out=A: lib.b200_top_distill_forward(A, tok, q, losses, out, A, need, 4, 5000, 5000, F32, 8, 1.0, None)
+    for change in ({"tok": four}, {"q": two}, {"losses": two}, {"out": four}):
+        assert fwd(**change) == 1, change
+    step = lambda tok=A, q=A, out=A: lib.b200_top_distill_step(A, tok, q, A, out, A, need, 4, 5000, 5000, F32, 8, 1.0, 1, None)
+    for change in ({"tok": four}, {"q": two}, {"out": four}):
+        assert step(**change) == 1, change
+    norm = lambda x=A, w=A, b=A, y=A: lib.b200_layer_norm(x, w, b, y, A, 4, 64, 64, F16, F32, 1e-5, None)
+    for change in ({"x": ODD}, {"y": ODD}, {"w": two}, {"b": two}):
+        assert norm(**change) == 1, change
+    n = lib.b200_layer_norm_scratch_bytes(4, 64)
+    grad = lambda x=A, w=A, dy=A, dx=A, dw=A, db=A: lib.b200_layer_norm_backward(x, w, A, dy, dx, dw, db, A, n, 4, 64, 64, 64, F16, F32, None)
+    for change in ({"x": ODD}, {"dy": ODD}, {"dx": ODD}, {"w": two}, {"dw": two}, {"db": two}):
+        assert grad(**change) == 1, change
+
+
 def test_cpu_tensors_are_refused():
     import pytorch_loss as P
     x, t = torch.randn(3, 10), torch.zeros(3, dtype=torch.int64)
