@@ -258,6 +258,9 @@ __device__ __forceinline__ void fill_slot(T *slot, const T *row, int D, int t, u
         const int tail = r.body + r.n;
         if (t < r.body) slot[off + t] = row[t];
         if (t < D - tail) slot[off + tail + t] = row[tail + t];
+        // The bulk copy that refills the slot may cover these bytes (its row starts elsewhere within 16 bytes): the
+        // threads that wrote them order their stores before it, the barrier in front of the refill does the rest.
+        if (t < r.body || t < D - tail) fence_proxy_async_smem();
     }
 }
 // Bytes of a slot: the row and the place of its first element in 16 bytes.
