@@ -25,6 +25,12 @@ def _prep(logits, top_tokens, top_logprobs, temperature):
     return (dev, top_tokens.contiguous(), top_logprobs.contiguous()) + _cabi.as_rows(logits)
 
 
+def _value(rec, reduction):
+    """The loss out of its record; no view in autograd's eyes, which would refuse `loss += other`.  (The record's
+    count, which backward reads, lies elsewhere in it.)"""
+    return rec[4 if reduction == 'mean' else 5].data
+
+
 # (allocations by new_empty: half the host time of torch.empty with a device)
 def _scratch(lib, q, rows, k):
     return q.new_empty(lib.b200_top_distill_scratch_bytes(rows, k) // 4)
@@ -92,14 +98,14 @@ class TopTokenDistillFunc(torch.autograd.Function):
             if step is not None:
                 rec, ctx.grad = step
                 ctx.save_for_backward(logits, top_tokens, top_logprobs)
-                return rec[4] if reduction == 'mean' else rec[5]
+                return _value(rec, reduction)
         losses, rec, scratch, flat, tok = _two_pass(logits, top_tokens, top_logprobs, temperature, reduction)
         if ctx.needs_input_grad[0]:
             shared = flat.data_ptr() == logits.data_ptr()
             ctx.kept = scratch, rec
             ctx.save_for_backward(logits if shared else flat, tok)
         if reduction in ('mean', 'sum'):
-            return rec[4] if reduction == 'mean' else rec[5]
+            return _value(rec, reduction)
         return losses
 
     @staticmethod
@@ -148,4 +154,4 @@ class TopTokenDistillLoss(nn.Module):
         if logits.requires_grad and torch.is_grad_enabled():
             return TopTokenDistillFunc.apply(logits, top_tokens, top_logprobs, float(self.temperature), self.reduction)
         losses, rec, _, _, _ = _two_pass(logits, top_tokens, top_logprobs, float(self.temperature), self.reduction)
-        return losses if rec is None else rec[4] if self.reduction == 'mean' else rec[5]
+        return losses if rec is None else _value(rec, self.reduction)

@@ -1,0 +1,45 @@
+"""The operators at a language model's output end where a program goes beyond their plain use: losses changed in place,
+forward-mode differentiation, batches without rows, what a call allocates, results that have to be exact."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _distill_inputs(rows=6, v=3000, k=4, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(v)
+    x = torch.randn(rows, v, generator=g, device="cuda").to(dtype)
+    tok = torch.randint(0, v, (rows, k), generator=g, device="cuda")
+    return x, tok, torch.randn(rows, k, generator=g, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_a_loss_may_be_changed_in_place(reduction, dtype):
+    """`loss += other` and `loss *= w`, as programs with several losses do; v = 500 takes two passes in every type.
+    Upstream gradients of 1 and 0.5 are powers of two: gradients are equal bit for bit."""
+    import pytorch_loss as P
+    crit = P.TopTokenDistillLoss(reduction=reduction)
+    for v in (500, 3000):
+        x, tok, q = _distill_inputs(v=v, dtype=dtype)
+        other = torch.ones((), device="cuda", requires_grad=True)
+        want_loss, want = [], []
+        for w in (1.0, 0.5):
+            leaf = x.clone().requires_grad_(True)
+            loss = crit(leaf, tok, q)
+            want_loss.append(loss.detach() * w + 1)
+            want += torch.autograd.grad(loss * w, leaf)
+        for w, wl, wg in zip((1.0, 0.5), want_loss, want):
+            leaf = x.clone().requires_grad_(True)
+            loss = crit(leaf, tok, q)
+            if w != 1.0:
+                loss *= w
+            loss += other
+            loss.backward()
+            assert torch.equal(loss.detach(), wl) and torch.equal(leaf.grad, wg)
+        assert float(other.grad) == 2.0
+        with torch.no_grad():
+            total = crit(x, tok, q)
+        total += other                                       # a loss taken without a graph, in a sum that has one
+        total.backward()
+        assert float(other.grad) == 3.0 and torch.equal(total.detach(), want_loss[0])
