@@ -11,6 +11,7 @@ import os
 import threading
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libb200loss.so")
@@ -256,6 +257,20 @@ def as_rows(t):
         if n > 1 and t.stride(-1) != 1:
             t = t.contiguous()
     return t, t.shape[0], n, t.stride(0)
+
+
+def tracked(*tensors):
+    """Whether autograd has to see a call: an input needs a gradient, or carries a tangent of forward mode -- which the
+    autograd functions refuse, as they have no such derivative; without them it would be dropped in silence."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:                      # (unpack_dual's own first look; it costs 0.4 us a tensor)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
 
 
 def once_differentiable(backward):

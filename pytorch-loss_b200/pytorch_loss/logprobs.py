@@ -111,7 +111,7 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0, ignore_index=-100):
     NaN.  Rows may lie apart in memory (`logits[..., :vocabulary]` of a padded head).
     """
     top_k, temperature, ignore_index = int(top_k), float(temperature), int(ignore_index)
-    if logits.requires_grad and torch.is_grad_enabled():
+    if _cabi.tracked(logits):
         return TokenLogProbs(*TokenLogProbsFunc.apply(logits, tokens, top_k, temperature, ignore_index))
     dev = _check(logits, tokens, top_k, temperature)
     return TokenLogProbs(*_forward(dev, logits, tokens, top_k, temperature, ignore_index, False)[2:6])

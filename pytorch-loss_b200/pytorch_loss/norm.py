@@ -83,8 +83,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     have the type of what they belong to.  Rows may lie apart in memory (one stride between them); the result is
     contiguous."""
     eps = float(eps)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
+    if _cabi.tracked(x, weight, bias):
         return LayerNormFunc.apply(x, weight, bias, eps)
     return _forward(x, weight, bias, eps, False)[0]
 

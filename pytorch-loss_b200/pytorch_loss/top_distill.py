@@ -151,7 +151,7 @@ class TopTokenDistillLoss(nn.Module):
         self.reduction = reduction
 
     def forward(self, logits, top_tokens, top_logprobs):
-        if logits.requires_grad and torch.is_grad_enabled():
+        if _cabi.tracked(logits):
             return TopTokenDistillFunc.apply(logits, top_tokens, top_logprobs, float(self.temperature), self.reduction)
         losses, rec, _, _, _ = _two_pass(logits, top_tokens, top_logprobs, float(self.temperature), self.reduction)
         return losses if rec is None else _value(rec, self.reduction)

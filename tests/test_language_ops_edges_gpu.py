@@ -43,3 +43,22 @@ def test_a_loss_may_be_changed_in_place(reduction, dtype):
         total += other                                       # a loss taken without a graph, in a sum that has one
         total.backward()
         assert float(other.grad) == 3.0 and torch.equal(total.detach(), want_loss[0])
+
+
+def test_forward_mode_is_refused():
+    """A tangent is never dropped in silence."""
+    import torch.autograd.forward_ad as fwAD
+    import pytorch_loss as P
+    x, tok, q = _distill_inputs()
+    w, b = torch.ones(3000, device="cuda"), torch.zeros(3000, device="cuda")
+    crit = P.TopTokenDistillLoss()
+    calls = [lambda d: P.token_logprobs(d(x), tok[:, 0]), lambda d: P.token_logprobs(d(x), tok[:, 0], top_k=3),
+             lambda d: crit(d(x), tok, q), lambda d: P.TopTokenDistillLoss(reduction='none')(d(x), tok, q),
+             lambda d: P.layer_norm(d(x), w, b), lambda d: P.layer_norm(x, d(w), b), lambda d: P.layer_norm(x, w, d(b)),
+             lambda d: P.layer_norm(d(x))]
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), fwAD.dual_level():
+            for call in calls:
+                with pytest.raises(NotImplementedError):
+                    call(lambda t: fwAD.make_dual(t, torch.ones_like(t)))
+                call(lambda t: t)                            # (no tangent: nothing to refuse)
