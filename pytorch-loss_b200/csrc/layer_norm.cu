@@ -515,10 +515,11 @@ __global__ void __launch_bounds__(ring_block<G>, backward_blocks<G>) norm_backwa
         load_columns<T, V, G>(x, own.n, t, h);
         load_columns<T, V, G>(dy, own.n, t, g);
         {
-            const pk_t nmr = psplat(-st.x * st.y), rr = psplat(st.y);
+            // (the difference first, as forward forms it: x r - mean r would be off by 2^-24 |mean| r in every column)
+            const pk_t negm = psplat(-st.x), rr = psplat(st.y);
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
-                h[i] = pfma(h[i], rr, nmr);
+                h[i] = pmul(padd(h[i], negm), rr);
                 dw[i] = pfma(g[i], h[i], dw[i]);
                 db[i] = padd(db[i], g[i]);
                 g[i] = pmul(g[i], w[i]);

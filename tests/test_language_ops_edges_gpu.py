@@ -62,3 +62,23 @@ def test_forward_mode_is_refused():
                 with pytest.raises(NotImplementedError):
                     call(lambda t: fwAD.make_dual(t, torch.ones_like(t)))
                 call(lambda t: t)                            # (no tangent: nothing to refuse)
+
+
+@pytest.mark.parametrize("dtype, par", [(torch.float32, torch.float32), (torch.float16, torch.float32),
+                                        (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("d", [256, 1024, 4096, 8192, 16384])
+def test_constant_rows_leave_the_weight_alone(d, dtype, par):
+    """Rows of one value c, of few bits, and d a power of two: every partial sum is exact (a share of 2^k values of at
+    most 24 - 14 bits), the mean is c and h = 0 exactly, so the weight's gradient is 0, y is the bias and a row's dx is
+    r (g - mean g) -- in the forward kernel's sense and in the backward kernel's."""
+    import pytorch_loss as P
+    c = torch.tensor([1000.0, -1004.0, 0.5, 120.0, 5.0], device="cuda").to(dtype)
+    x = c.unsqueeze(1).expand(5, d).contiguous().requires_grad_(True)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    w = torch.randn(d, generator=g, device="cuda").to(par).requires_grad_(True)
+    b = torch.randn(d, generator=g, device="cuda").to(par).requires_grad_(True)
+    dy = torch.randn(5, d, generator=g, device="cuda").to(dtype)
+    y = P.layer_norm(x, w, b)
+    assert torch.equal(y.detach(), b.detach().to(dtype).expand(5, d))
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert float(dw.abs().max()) == 0.0
