@@ -398,11 +398,12 @@ extern "C" int b200_top_distill_forward(const void *logits, const int64_t *top_t
     const char *who = "b200_top_distill_forward";
     if (const int rc = check_distill(who, logits, top_tokens, scratch, scratch_bytes, rows, V, stride, dtype, K, temperature))
         return rc;
-    if ((rows > 0 && !top_logprobs) || (!losses && !out) || !lies_on(top_logprobs, 4) || !lies_on(losses, 4) ||
+    if ((rows > 0 && (!top_logprobs || (!losses && !out))) || !lies_on(top_logprobs, 4) || !lies_on(losses, 4) ||
         !lies_on(out, 8)) {
         set_error("%s: null or misaligned pointer", who);
         return B200_ERR_ARG;
     }
+    if (rows == 0 && !out) return B200_OK;                  // (no rows' losses: an empty tensor has no address)
     const DistillScratch d = carve(scratch, rows);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (const int rc = launch_lists(top_tokens, top_logprobs, d, rows, K, int(V), s)) return rc;

@@ -1,4 +1,6 @@
 """The operators at a language model's output end: host logic of what lies beyond their plain use, on the CPU."""
+import ctypes
+
 import torch
 import torch.autograd.forward_ad as fwAD
 
@@ -15,3 +17,17 @@ def test_which_calls_autograd_has_to_see():
         for grad in (True, False):
             with torch.set_grad_enabled(grad):
                 assert _cabi.tracked(dual) and _cabi.tracked(x, None, dual) and not _cabi.tracked(x)
+
+
+def test_no_rows_need_no_address_for_their_losses():
+    """An empty tensor's pointer is null: the losses of no rows are nothing to do, not an error."""
+    import build as b200_build
+    b200_build.build()
+    from pytorch_loss import _cabi
+    lib = _cabi.load_library()
+    made_up = ctypes.c_void_p(0x7f0000001000)               # (never used: there is nothing to do)
+    need = lib.b200_top_distill_scratch_bytes(0, 4)
+    call = lambda rows: lib.b200_top_distill_forward(None if rows == 0 else made_up, None if rows == 0 else made_up,
+                                                     None if rows == 0 else made_up, None, None, made_up, 1 << 20, rows,
+                                                     100, 100, _cabi.F32, 4, 1.0, None)
+    assert need <= 1 << 20 and call(0) == 0 and call(3) == 1

@@ -82,3 +82,19 @@ def test_constant_rows_leave_the_weight_alone(d, dtype, par):
     assert torch.equal(y.detach(), b.detach().to(dtype).expand(5, d))
     dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
     assert float(dw.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("v", [30, 3000])
+def test_no_rows_give_no_losses(v, dtype):
+    import pytorch_loss as P
+    crit = P.TopTokenDistillLoss(reduction='none')
+    for shape in ((0,), (0, 3), (3, 0)):
+        x = torch.zeros(shape + (v,), device="cuda", dtype=dtype)
+        lists = torch.zeros(shape + (4,), dtype=torch.int64, device="cuda"), torch.zeros(shape + (4,), device="cuda")
+        assert crit(x, *lists).shape == shape
+        x.requires_grad_(True)
+        losses = crit(x, *lists)
+        assert losses.shape == shape and losses.dtype == torch.float32
+        losses.sum().backward()
+        assert x.grad.shape == x.shape
