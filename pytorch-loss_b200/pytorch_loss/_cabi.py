@@ -19,7 +19,6 @@ LIB_PATH = os.path.join(_HERE, "libb200loss.so")
 ABI_VERSION = 3
 STEP_DEFER, STEP_AFTER_COUNT = 1, 2      # bits of the fused steps' `defer` argument (b200loss.h)
 F32, F16, BF16, F64 = 0, 1, 2, 3
-UNSUPPORTED = 2                          # B200_ERR_UNSUPPORTED
 
 _c = ctypes
 _vp, _i64, _int, _f32, _f64, _sz = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_float, _c.c_double, _c.c_size_t

@@ -68,18 +68,16 @@ def _step(logits, top_tokens, top_logprobs, temperature, reduction):
     """(record, final gradient) from one read of the logits, or None when this layout has no such step."""
     dev, tok, q, flat, rows, v, stride = _prep(logits, top_tokens, top_logprobs, temperature)
     lib, k, dt = _cabi.load_library(), tok.shape[-1], _cabi.dtype_code(flat)
-    if dt == _cabi.F16 or rows == 0:
+    # (asked before the gradient is allocated, whose address ends in zeros as 0 does)
+    if not lib.b200_top_distill_step_path(flat.data_ptr(), None, rows, v, stride, dt):
         return None
     grad = flat.new_empty(logits.shape)
     scratch = _scratch(lib, q, rows, k)
     rec = q.new_empty(8)
     with _cabi.on_device(dev):
-        code = lib.b200_top_distill_step(
+        _cabi.check(lib.b200_top_distill_step(
             flat.data_ptr(), tok.data_ptr(), q.data_ptr(), grad.data_ptr(), rec.data_ptr(), scratch.data_ptr(),
-            4 * scratch.numel(), rows, v, stride, dt, k, temperature, int(reduction == 'mean'), _cabi.stream_ptr(dev))
-    if code == _cabi.UNSUPPORTED:
-        return None
-    _cabi.check(code)
+            4 * scratch.numel(), rows, v, stride, dt, k, temperature, int(reduction == 'mean'), _cabi.stream_ptr(dev)))
     return rec, grad
 
 

@@ -98,3 +98,21 @@ def test_no_rows_give_no_losses(v, dtype):
         assert losses.shape == shape and losses.dtype == torch.float32
         losses.sum().backward()
         assert x.grad.shape == x.shape
+
+
+@pytest.mark.parametrize("rows, v, pad, dtype", [(64, 131072, 0, torch.float32), (4000, 1000, 0, torch.float32),
+                                                 (500, 20001, 47, torch.bfloat16)])
+def test_a_layout_without_the_step_allocates_no_gradient_forward(rows, v, pad, dtype):
+    """Rows above 320 KB or up to 4 KB, rows off the gradient's place: two passes.  Forward keeps 24 + 4 K bytes a row."""
+    import pytorch_loss as P
+    x, tok, q = _distill_inputs(rows, v + pad, 4, dtype)
+    leaf = x[:, :v].requires_grad_(True)
+    tok = tok.clamp(max=v - 1)
+    crit = P.TopTokenDistillLoss()
+    crit(leaf, tok, q)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    loss = crit(leaf, tok, q)
+    assert torch.cuda.max_memory_allocated() - before < leaf.numel() * leaf.element_size() // 4
+    loss.backward()
