@@ -448,9 +448,12 @@ int b200_token_logprobs_backward(const void *logits, const int64_t *tokens, cons
  *   step    : out and the final gradient (mean: divided by the number of counted rows) from ONE read of
  *       the logits; b200_top_distill_step_path: 1 when the layout has it (float32 / bfloat16, gradient
  *       rows at the logits' place within 16 bytes, rows of more than 4 KB and up to 320 KB; others are as
- *       fast in two passes).  float16 has none: there the
- *       upstream gradient (loss scaling) has to come in before the one rounding.  Backward of the step is
- *       b200_rescale_gradient.
+ *       fast in two passes).  float16 has none: its gradients often need a loss scale, which has to come
+ *       in before the one rounding, and a step would write them twice
+ *       Backward of a float32 step is b200_rescale_gradient
+ *   step_backward: a bfloat16 step's gradient times *d_loss, in place and with one rounding: nothing to
+ *       do when that is 1, else written again from the logits and what the step left in scratch.  count:
+ *       the record's for a mean, null for a sum
  * scratch: b200_top_distill_scratch_bytes(rows, K) bytes, 16-byte aligned, contents irrelevant. */
 size_t b200_top_distill_scratch_bytes(int64_t rows, int K);
 int b200_top_distill_forward(const void *logits, const int64_t *top_tokens, const float *top_logprobs,
@@ -467,6 +470,10 @@ int b200_top_distill_step(const void *logits, const int64_t *top_tokens, const f
                           void *grad_logits, void *out, void *scratch, size_t scratch_bytes,
                           int64_t rows, int64_t V, int64_t stride, int dtype, int K, float temperature,
                           int mean, void *stream);
+int b200_top_distill_step_backward(const void *logits, const int64_t *top_tokens, const void *scratch,
+                                   size_t scratch_bytes, const float *d_loss, const void *count,
+                                   void *grad_logits, int64_t rows, int64_t V, int64_t stride, int dtype,
+                                   int K, float temperature, void *stream);
 
 /* ------------------------------------------------------------------ layer norm ---
  * Rows of D contiguous elements (row r at element r * stride of x, any alignment), at most 2^31 - 1 rows

@@ -543,11 +543,10 @@ struct TokenGradParams {
 // G threads to a chunk of G * kTokenUnroll vectors.  ALIGNED: logits and gradient rows start at the same place within
 // 16 bytes, so that whole vectors of one are whole vectors of the other; else the logits are read one by one.
 template <typename T, int G, int MODE, bool ALIGNED>
-__global__ void __launch_bounds__(256) token_grad_kernel(const TokenGradParams p) {
+__device__ __forceinline__ void token_grad_chunk(const TokenGradParams &p, unsigned unit) {
     constexpr int N = TokenVec<T>::N;
     constexpr int GROUPS = 256 / G;
     const int t = threadIdx.x % G;
-    const unsigned unit = blockIdx.x * GROUPS + threadIdx.x / G;
     const int64_t r = G == 32 ? unit : unit / unsigned(p.chunks);
     const int chunk = G == 32 ? 0 : int(unit % unsigned(p.chunks));
     if (r >= p.rows) return;
@@ -651,6 +650,10 @@ __global__ void __launch_bounds__(256) token_grad_kernel(const TokenGradParams p
         g[j] = from_f32<T>(d[0].x);
     }
 }
+template <typename T, int G, int MODE, bool ALIGNED>
+__global__ void __launch_bounds__(256) token_grad_kernel(const TokenGradParams p) {
+    token_grad_chunk<T, G, MODE, ALIGNED>(p, blockIdx.x * (256 / G) + threadIdx.x / G);
+}
 
 // ---- launches
 
@@ -687,6 +690,9 @@ template <typename T, int MODE, bool TOP> int launch_stats(const TokenParams &pr
                           p);
 }
 
+// Chunks of a row of so many vectors, 256 threads to a chunk.
+inline int grad_chunks(int64_t vectors) { return int((vectors + 256 * kTokenUnroll - 1) / (256 * kTokenUnroll)); }
+
 template <typename T, int MODE> int launch_grad(const TokenGradParams &prm, int dtype, cudaStream_t stream) {
     TokenGradParams p = prm;
     const char *what = "token gradient kernel launch";
@@ -700,7 +706,7 @@ template <typename T, int MODE> int launch_grad(const TokenGradParams &prm, int 
         return aligned ? launch_cluster(token_grad_kernel<T, 32, MODE, true>, grid, 256, 0, 1, false, stream, what, p)
                        : launch_cluster(token_grad_kernel<T, 32, MODE, false>, grid, 256, 0, 1, false, stream, what, p);
     }
-    p.chunks = int((vectors + 256 * kTokenUnroll - 1) / (256 * kTokenUnroll));
+    p.chunks = grad_chunks(vectors);
     const int64_t grid = p.rows * p.chunks;
     if (grid > 0x7fffffff) {
         set_error("%s: %lld rows of %d logits are more than one launch covers", what, (long long)p.rows, p.V);

@@ -161,6 +161,7 @@ struct StepParams {
     const float *weight, *base;
     const int *counts;          // the rows of a mean, in kListSlots parts; null: a sum
     float *losses;
+    float4 *stats;              // what the gradient needs if it has to be written again
 };
 
 // One row per block (HELD: copied to shared memory once, in pieces, and read twice there) or per cluster of up to two
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(THREADS) distill_step_kernel(const StepParams 
     constexpr int N = TokenVec<T>::N, WARPS = THREADS / 32;
     extern __shared__ __align__(16) uint4 held[];
     __shared__ uint64_t full[kStepPieces];
-    __shared__ float wm[WARPS], wsum[WARPS], wloss[WARPS], joined[3];
+    __shared__ float wm[WARPS], wsum[WARPS], wloss[WARPS], joined[3], of_row[2];
     __shared__ int wcount[WARPS];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int parts = 1 << p.part_shift, rank = int(blockIdx.x) & (parts - 1);
@@ -256,6 +257,10 @@ __global__ void __launch_bounds__(THREADS) distill_step_kernel(const StepParams 
 
     const float m = reference_of(st.m), log2s = log2f(st.s);
     const bool nothing = st.s == 0.f;
+    if (t == 0) {                                           // (out of the registers that the loop below wants)
+        of_row[0] = m;
+        of_row[1] = st.s;
+    }
     float scale = p.inv_t;
     if (p.counts) scale /= float(count);
     if (base != base) scale = base;
@@ -306,10 +311,23 @@ __global__ void __launch_bounds__(THREADS) distill_step_kernel(const StepParams 
         if (rank == 0 && t == 0) {
             for (int i = 1; i < parts; ++i) loss += cluster.map_shared_rank(&joined[0], i)[2];
         }
-        if (rank == 0 && t == 0) p.losses[r] = base + loss;
         cluster.sync();                                     // (nobody leaves while its memory is read)
-    } else if (t == 0) {
+    }
+    if (rank == 0 && t == 0) {
+        const float s = of_row[1];
         p.losses[r] = base + loss;
+        p.stats[r] = make_float4(of_row[0], s == 0.f ? 0.f : 1.f / s, 0.f, log2f(s));
+    }
+}
+
+// Behind a bfloat16 step: its gradient for an upstream gradient other than 1, from the logits and what the step left.  As
+// many bytes as scaling the written gradient would move, but one rounding.  A grid of what runs at once goes through the
+// chunks, so that it costs 2 us to find that the upstream gradient is 1.
+__global__ void __launch_bounds__(256) distill_again_kernel(const TokenGradParams p, unsigned chunks) {
+    if (*p.d_out == 1.f) return;
+    for (unsigned i = blockIdx.x; i < chunks; i += gridDim.x) {
+        token_grad_chunk<__nv_bfloat16, 256, kList, true>(p, i);
+        __syncthreads();                                    // (the chunk's list is in shared memory)
     }
 }
 
@@ -382,6 +400,28 @@ int check_distill(const char *who, const void *x, const int64_t *tokens, const v
     return B200_OK;
 }
 
+TokenGradParams grad_params(const void *logits, const int64_t *top_tokens, const void *scratch, const float *d_loss, int per_row,
+                            const void *count, void *grad, int64_t rows, int64_t V, int64_t stride, int K, float temperature) {
+    const DistillScratch d = carve(const_cast<void *>(scratch), rows);
+    TokenGradParams p{};
+    p.x = logits;
+    p.grad = grad;
+    p.stride = stride;
+    p.rows = rows;
+    p.V = int(V);
+    p.inv_t = 1.f / temperature;
+    p.c = float(1.4426950408889634 / double(temperature));
+    p.ids = top_tokens;
+    p.weight = d.weight;
+    p.base = d.base;
+    p.stats = d.stats;
+    p.d_out = d_loss;
+    p.d_out_step = per_row ? 1 : 0;
+    p.count = static_cast<const double *>(count);
+    p.K = K;
+    return p;
+}
+
 }  // namespace
 }  // namespace b200
 
@@ -439,23 +479,8 @@ extern "C" int b200_top_distill_backward(const void *logits, const int64_t *top_
         set_error("%s: null or misaligned pointer", who);
         return B200_ERR_ARG;
     }
-    const DistillScratch d = carve(const_cast<void *>(scratch), rows);
-    TokenGradParams p{};
-    p.x = logits;
-    p.grad = grad_logits;
-    p.stride = stride;
-    p.rows = rows;
-    p.V = int(V);
-    p.inv_t = 1.f / temperature;
-    p.c = float(1.4426950408889634 / double(temperature));
-    p.ids = top_tokens;
-    p.weight = d.weight;
-    p.base = d.base;
-    p.stats = d.stats;
-    p.d_out = d_loss;
-    p.d_out_step = per_row ? 1 : 0;
-    p.count = static_cast<const double *>(count);
-    p.K = K;
+    const TokenGradParams p = grad_params(logits, top_tokens, scratch, d_loss, per_row, count, grad_logits, rows, V, stride, K,
+                                          temperature);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return dtype == B200_F32   ? launch_grad<float, kList>(p, dtype, s)
            : dtype == B200_F16 ? launch_grad<__half, kList>(p, dtype, s)
@@ -503,7 +528,34 @@ extern "C" int b200_top_distill_step(const void *logits, const int64_t *top_toke
     p.base = d.base;
     p.counts = mean ? d.counts : nullptr;
     p.losses = d.losses;
+    p.stats = d.stats;
     const int rc = dtype == B200_F32 ? launch_step<float>(p, dtype, s) : launch_step<__nv_bfloat16>(p, dtype, s);
     if (rc) return rc;
     return launch_finish(d.losses, d.counts, rows, out, s);
+}
+
+extern "C" int b200_top_distill_step_backward(const void *logits, const int64_t *top_tokens, const void *scratch,
+                                              size_t scratch_bytes, const float *d_loss, const void *count,
+                                              void *grad_logits, int64_t rows, int64_t V, int64_t stride, int dtype, int K,
+                                              float temperature, void *stream) {
+    const char *who = "b200_top_distill_step_backward";
+    if (const int rc = check_distill(who, logits, top_tokens, scratch, scratch_bytes, rows, V, stride, dtype, K, temperature))
+        return rc;
+    if (!d_loss || !lies_on(d_loss, 4) || !lies_on(count, 8)) {
+        set_error("%s: null or misaligned pointer", who);
+        return B200_ERR_ARG;
+    }
+    if (dtype != B200_BF16 || !grad_logits || !b200_top_distill_step_path(logits, grad_logits, rows, V, stride, dtype)) {
+        set_error("%s: need bfloat16 logits that have a one-pass step", who);
+        return B200_ERR_UNSUPPORTED;
+    }
+    TokenGradParams p = grad_params(logits, top_tokens, scratch, d_loss, 0, count, grad_logits, rows, V, stride, K, temperature);
+    p.chunks = grad_chunks(row_vectors(V, dtype));
+    const int64_t chunks = rows * p.chunks, most = int64_t(sm_count()) * 6;
+    if (chunks > 0x7fffffff) {
+        set_error("%s: %lld rows of %d logits are more than one launch covers", who, (long long)rows, p.V);
+        return B200_ERR_UNSUPPORTED;
+    }
+    return launch_cluster(distill_again_kernel, chunks < most ? chunks : most, 256, 0, 1, false,
+                          static_cast<cudaStream_t>(stream), "distillation gradient kernel launch", p, unsigned(chunks));
 }

@@ -83,6 +83,7 @@ SIGNATURES = {
     "b200_top_distill_backward": (_int, [_vp, _vp, _vp, _sz, _vp, _int, _vp, _vp, _i64, _i64, _i64, _int, _int, _f32, _vp]),
     "b200_top_distill_step_path": (_int, [_vp, _vp, _i64, _i64, _i64, _int]),
     "b200_top_distill_step": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _i64, _int, _int, _f32, _int, _vp]),
+    "b200_top_distill_step_backward": (_int, [_vp, _vp, _vp, _sz, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _f32, _vp]),
 }
 
 _lib = None

@@ -116,3 +116,59 @@ def test_a_layout_without_the_step_allocates_no_gradient_forward(rows, v, pad, d
     loss = crit(leaf, tok, q)
     assert torch.cuda.max_memory_allocated() - before < leaf.numel() * leaf.element_size() // 4
     loss.backward()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("v", [2056, 9000, 32768, 50001, 131072])
+def test_a_scaled_gradient_is_rounded_once(v, reduction):
+    """The one-pass step in bfloat16 under an upstream gradient that is no power of two: half a step of the type and what
+    its float32 arithmetic loses, as without one.  The second trip through the graph gives the same bits."""
+    import pytorch_loss as P
+    from test_top_distill_gpu import U, close, expected, inputs
+    x, tok, q = inputs(300, v, 20, torch.bfloat16, seed=v, ragged=True)
+    _, grad, counted, _, gtol = expected(x, tok, q, 1.25)
+    scale = 0.3 / (int(counted.sum()) if reduction == "mean" else 1)
+    leaf = x.detach().requires_grad_(True)
+    loss = P.TopTokenDistillLoss(1.25, reduction)(leaf, tok, q)
+    up = torch.tensor(0.3, device="cuda")
+    got, = torch.autograd.grad(loss, leaf, up, retain_graph=True)
+    want = grad * scale
+    close(got, want, gtol * scale + want.abs() * (torch.finfo(torch.bfloat16).eps / 2 + 8 * U) + 2.0 ** -126, "gradient")
+    again, = torch.autograd.grad(loss, leaf, up)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("rows", [5, 4000])
+def test_a_step_under_one_upstream_gradient_then_another(rows):
+    """A captured backward pass is replayed with upstream gradients of 1, 0.3 and 1 again: each replay gives what an
+    eager call gives."""
+    import pytorch_loss as P
+    x, tok, q = _distill_inputs(rows, 5001, 7, torch.bfloat16)
+    crit, up = P.TopTokenDistillLoss(), torch.ones((), device="cuda")
+    leaf = x.clone().requires_grad_(True)
+    call = lambda: torch.autograd.grad(crit(leaf, tok, q), leaf, up)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for value in (1.0, 0.3, 1.0):
+        up.fill_(value)
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, call())
+
+
+def test_steps_notice_changed_logits():
+    """What a bfloat16 step's backward may have to read again must not have changed meanwhile."""
+    import pytorch_loss as P
+    x, tok, q = _distill_inputs(6, 5001, 4, torch.bfloat16)
+    y = x.requires_grad_(True) * 1
+    loss = P.TopTokenDistillLoss()(y, tok, q)
+    with torch.no_grad():
+        y.add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        loss.backward()
