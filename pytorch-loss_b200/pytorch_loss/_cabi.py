@@ -245,14 +245,18 @@ def split_shape(logits, labels=None):
 def as_rows(t):
     """(tensor whose memory the kernels read, rows, n, elements from row to row) of a tensor [..., n].  Rows may lie
     apart (a slice of a padded storage, a permuted view) as long as one stride describes them; anything else is copied."""
-    if t.dim() < 1 or t.shape[-1] == 0:
-        raise RuntimeError("need a tensor [..., n] with n > 0, got shape %s" % (tuple(t.shape),))
-    n = t.shape[-1]
+    shape = t.shape
+    dims = len(shape)
+    if dims < 1 or shape[-1] == 0:
+        raise RuntimeError("need a tensor [..., n] with n > 0, got shape %s" % (tuple(shape),))
+    n = shape[-1]
     if n > 1 and t.stride(-1) != 1:
         t = t.contiguous()
-    if t.dim() == 1:
+    if dims == 2:
+        return t, shape[0], n, t.stride(0)
+    if dims == 1:
         t = t.unsqueeze(0)
-    elif t.dim() > 2:
+    else:
         t = t.flatten(0, -2)
         if n > 1 and t.stride(-1) != 1:
             t = t.contiguous()
