@@ -439,7 +439,9 @@ int b200_token_logprobs_backward(const void *logits, const int64_t *tokens, cons
  * No counterpart in the reference.  Logits as above against lists of K <= 128 tokens with log
  * probabilities (top_tokens, top_logprobs [rows, K], as b200_token_logprobs writes them):
  *   w = softmax(top_logprobs[r, :])     loss[r] = sum_k w_k (log w_k - log p[top_tokens[r, k]])
- * Entries with a negative token do not exist, the same token twice adds up.  A row without an entry of
+ * Entries with a negative token do not exist; of a token that stands in the list twice both terms count in
+ * the loss, and its weight in the gradient is the sum of both.  The temperature is the student's: lists are
+ * taken as they are, and there is no factor T^2.  A row without an entry of
  * finite log probability is not read: loss 0, gradient 0, not counted.  A token >= V gives NaN.
  *   forward : losses float[rows] and / or out (reduction record: sum, count, mean over the counted rows)
  *   backward: grad_logits [rows, V] contiguous = d_loss (p_j - w_j) / T, d_loss one float per row
@@ -447,8 +449,8 @@ int b200_token_logprobs_backward(const void *logits, const int64_t *tokens, cons
  *       scratch: what the forward call of the same inputs left
  *   step    : out and the final gradient (mean: divided by the number of counted rows) from ONE read of
  *       the logits; b200_top_distill_step_path: 1 when the layout has it (float32 / bfloat16, gradient
- *       rows at the logits' place within 16 bytes, rows of more than 4 KB and up to 320 KB; others are as
- *       fast in two passes).  float16 has none: its gradients often need a loss scale, which has to come
+ *       rows at the logits' place within 16 bytes, rows of more than 4 KB and up to 320 KB; shorter rows are
+ *       as fast in two passes).  float16 has none: its gradients often need a loss scale, which has to come
  *       in before the one rounding, and a step would write them twice
  *       Backward of a float32 step is b200_rescale_gradient
  *   step_backward: a bfloat16 step's gradient times *d_loss, in place and with one rounding: nothing to

@@ -9,9 +9,12 @@
 // block order, so results repeat bit for bit.
 //
 // Bound: HBM (2 s D per row forward, 3 s D backward, s the element's bytes).  Measured, us and share of the 6.55 TB/s of
-// a copy:  [16384, 4096] bfloat16, float32 weights   50 (0.81) + 78 (0.79)     [16384, 8192] float16   90 (0.91) + 147 (0.84)
-//          [32768, 2048] float32                     82 (0.99) + 141 (0.87)    [16384, 4001] float32   96 (0.83) + 146 (0.82)
-// Rows of odd widths in 16 bits go element by element and reach 0.36.
+// a copy:  [16384, 4096] bfloat16, float32 weights   50 (0.82) + 80 (0.77)     [16384, 8192] float16   90 (0.91) + 151 (0.81)
+//          [32768, 2048] float32                     81 (1.01) + 137 (0.90)    [16384, 4001] float32   92 (0.87) + 150 (0.80)
+//          [4096, 12288] bfloat16                    39 (0.78) + 113 (0.41)    [8192, 16384] float32  226 (0.73) + 309 (0.80)
+// Beyond 8192 columns backward waits for a cluster's barrier in every row (2 us).  16-bit rows that are not whole vectors
+// go element by element ([16384, 4001] float16 89 (0.45) + 139 (0.43)), forward rows beyond 64 KB in three sweeps
+// ([1024, 40000] bfloat16 84, 0.30).
 #include <algorithm>
 
 #include "token_rows.cuh"
@@ -29,7 +32,7 @@ struct NormParams {
     int blocks, share;          // blocks of a cluster that share a row, and columns of each (the last one: what is left)
     float eps;
 };
-constexpr int kMaxStages = 8;
+constexpr int kMaxSlots = 8;
 constexpr size_t kRingBytes = 200 * 1024;     // of an SM's shared memory
 
 // V elements of T as floats.
@@ -354,7 +357,7 @@ template <typename T, typename P, int G>
 __global__ void __launch_bounds__(ring_block<G>, forward_blocks<G>) norm_forward_ragged_kernel(const NormParams p) {
     constexpr int GROUPS = ring_block<G> / G, WARPS = G / 32;
     extern __shared__ __align__(16) char slots[];
-    __shared__ uint64_t full[GROUPS][kMaxStages];
+    __shared__ uint64_t full[GROUPS][kMaxSlots];
     __shared__ float2 moments[GROUPS][2][WARPS];            // {mean, sum of squares around it} of each warp's columns
     __shared__ int lost[GROUPS];
     const int t = threadIdx.x % G, group = threadIdx.x / G, lane = threadIdx.x & 31, warp = t >> 5;
@@ -465,7 +468,7 @@ template <typename T, typename P, int V, int G>
 __global__ void __launch_bounds__(ring_block<G>, backward_blocks<G>) norm_backward_kernel(const NormParams p) {
     constexpr int GROUPS = ring_block<G> / G, WARPS = G / 32;
     extern __shared__ __align__(16) char slots[];
-    __shared__ uint64_t full[GROUPS][kMaxStages];
+    __shared__ uint64_t full[GROUPS][kMaxSlots];
     __shared__ float2 sums[GROUPS][2][sum_slots<G>];
     __shared__ int lost[GROUPS];
     const int t = threadIdx.x % G, group = threadIdx.x / G, lane = threadIdx.x & 31, warp = t >> 5;
@@ -685,7 +688,7 @@ inline RingPlan ring_plan(int D, size_t s, bool backward) {
     if (r.threads <= 256) r.per_sm = backward ? 2 : 3;
     // (at least two slots: 8192 columns of x and dy in float32 are 64 KB)
     r.stages = int(kRingBytes / r.per_sm / (slot_bytes(r.share, s) * (backward ? 2 : 1) * r.groups()));
-    if (r.stages > kMaxStages) r.stages = kMaxStages;
+    if (r.stages > kMaxSlots) r.stages = kMaxSlots;
     return r;
 }
 // Teams of blocks that share a row.

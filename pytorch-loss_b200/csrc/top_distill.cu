@@ -341,6 +341,9 @@ __global__ void __launch_bounds__(256) distill_again_kernel(const TokenGradParam
 //   [4096, 131072] bfloat16 (256 KB)                                         479               488, by two blocks 408
 //   [2048, 81920] float32 (320 KB)                                           312               311, by two blocks 287
 //   [2048, 131072] float32 (512 KB)                                          478               532, by two blocks 529
+// With few rows a step leaves SMs idle where two passes split the rows, but both are short of what the host needs for the
+// call: [8, 80000] bfloat16 11 against 8, [148, 80000] 14 against 21, [8, 32768] 8 against 8.
+// Rows off the gradient's place within 16 bytes have no step: [8192, 50257] bfloat16 with rows of 50304 482 against 302.
 // From L2 works while the rows under way fit there (three blocks of 512 threads an SM: 57 MB at 128 KB, where 12 % of
 // the rows are read from memory twice).  What the step loses there it loses to its phases: a block reads, joins, writes.
 enum StepWay { kNoStep, kHeld128, kHeld256, kFromL2, kFromL2Pair };

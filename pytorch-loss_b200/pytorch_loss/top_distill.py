@@ -130,8 +130,10 @@ class TopTokenDistillLoss(nn.Module):
         >>> loss = criteria(student_logits, best.top_tokens, best.top_logprobs)     # [..., V], [..., K], [..., K]
 
     The teacher's probabilities are made to sum to one over each list; the student's are softmax(logits /
-    temperature).  Entries with a negative token do not exist (lists of any length in one tensor), the same token
-    twice adds up, a token beyond the vocabulary gives NaN.  A row without any entry -- or with log probabilities of
+    temperature).  The temperature is the student's alone: lists are taken as they are (for both sides at T take them by
+    `token_logprobs(..., temperature=T)`), and losses are not multiplied by T^2.  Entries with a negative token do not
+    exist (lists of any length in one tensor); of a token that stands in a list twice both terms count in the loss, and
+    its weight in the gradient is the sum; a token beyond the vocabulary gives NaN.  A row without any entry -- or with log probabilities of
     -inf only -- costs nothing, has no gradient and does not count in the 'mean' (NaN if there is none that counts).
     'mean' and 'sum' give a float32 scalar, anything else the rows' losses.  The teacher's side has no gradient.
     """
