@@ -449,10 +449,10 @@ int b200_token_logprobs_backward(const void *logits, const int64_t *tokens, cons
  *       scratch: what the forward call of the same inputs left
  *   step    : out and the final gradient (mean: divided by the number of counted rows) from ONE read of
  *       the logits; b200_top_distill_step_path: 1 when the layout has it (float32 / bfloat16, gradient
- *       rows at the logits' place within 16 bytes, rows of more than 4 KB and up to 320 KB; shorter rows are
- *       as fast in two passes).  float16 has none: its gradients often need a loss scale, which has to come
- *       in before the one rounding, and a step would write them twice
- *       Backward of a float32 step is b200_rescale_gradient
+ *       rows at the logits' place within 16 bytes, rows of more than 4 KB and up to 320 KB; shorter and
+ *       longer ones are as fast in two passes).  float16 has none: its gradients often need a loss scale,
+ *       which has to come in before the one rounding, and a step would write them twice.  Backward of a
+ *       float32 step is b200_rescale_gradient
  *   step_backward: a bfloat16 step's gradient times *d_loss, in place and with one rounding: nothing to
  *       do when that is 1, else written again from the logits and what the step left in scratch.  count:
  *       the record's for a mean, null for a sum

@@ -172,3 +172,21 @@ def test_steps_notice_changed_logits():
         y.add_(1)
     with pytest.raises(RuntimeError, match="inplace"):
         loss.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("v, pad", [(3000, 8), (5001, 3), (700, 4)])
+def test_saved_tensors_may_move(v, pad, dtype):
+    """What backward reads comes from autograd's saved tensors, wherever hooks have put them and with whatever strides."""
+    import pytorch_loss as P
+    x, tok, q = _distill_inputs(50, v + pad, 6, dtype)
+    tok, leaf = tok.clamp(max=v - 1), x.requires_grad_(True)
+    w, b = torch.randn(v, device="cuda"), torch.randn(v, device="cuda")
+    up, d, dy = torch.tensor(0.3, device="cuda"), torch.randn(50, device="cuda"), torch.randn(50, v, device="cuda").to(dtype)
+    for call, g in ((lambda y: P.TopTokenDistillLoss()(y, tok, q), up), (lambda y: P.token_logprobs(y, tok[:, 0]).logprobs, d),
+                    (lambda y: P.layer_norm(y, w, b), dy)):
+        want, = torch.autograd.grad(call(leaf[:, :v]), leaf, g)
+        with torch.autograd.graph.save_on_cpu():
+            out = call(leaf[:, :v])
+        got, = torch.autograd.grad(out, leaf, g)
+        assert torch.equal(got, want)
